@@ -4,6 +4,8 @@
 
 -ffp-contract=off is part of the numerical contract (no FMA contraction: IoU, box
 conversion and encode/decode round exactly like the fp32 reference arithmetic).
+-packed-fp32-ops keeps the compiler from pairing fp32 operations into packed instructions, some forms of which
+have given wrong results on this hardware now and then.
 """
 import glob
 import os
@@ -15,7 +17,8 @@ HERE = os.path.dirname(os.path.abspath(__file__))
 CSRC = os.path.join(HERE, 'csrc')
 OUT = os.path.join(HERE, 'libdetbox.so')
 OBJ = os.path.join(HERE, 'csrc', '_obj')
-FLAGS = ['--offload-arch=gfx950', '-O3', '-std=c++17', '-fPIC', '-ffp-contract=off', '-Wall', '-Wno-unused-function']
+FLAGS = ['--offload-arch=gfx950', '-O3', '-std=c++17', '-fPIC', '-ffp-contract=off', '-Xclang', '-target-feature', '-Xclang',
+         '-packed-fp32-ops', '-Wall', '-Wno-unused-function']
 
 
 def sources():
