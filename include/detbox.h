@@ -154,6 +154,73 @@ int detbox_smooth_l1_masked_forward(const float *input, const float *target, con
 int detbox_smooth_l1_masked_backward(const float *input, const float *target, const int64_t *labels,
                                      int64_t rows, const float *grad_scale, float *grad_input, void *stream);
 
+/* ---- class heads over many labels: normalise, multiply, log probabilities ------------------- */
+
+/* The operators of this section take fp32, bfloat16 or fp16 (`dtype`), rows of any length with a row stride (`ld*`, in
+ * elements, at least the row length) and no alignment beyond the element's own.  Outputs are dense.  Sums, statistics and
+ * products are fp32; every output is rounded once.  No entry point uses atomics or clears memory: results do not change
+ * from call to call, and every call can be captured into a HIP graph.  No counterpart in the reference, whose heads
+ * are convolutions of a few classes (src/models/retinanet.py:63-118). */
+#define DETBOX_F32 0
+#define DETBOX_BF16 1
+#define DETBOX_F16 2
+
+#define DETBOX_ACTIVATION_NONE 0
+#define DETBOX_ACTIVATION_RELU 1
+#define DETBOX_ACTIVATION_GELU 2    /* z * Phi(z), Phi the normal distribution function */
+#define DETBOX_ACTIVATION_SILU 3    /* z * sigmoid(z) */
+#define DETBOX_ACTIVATION_SIGMOID 4
+
+#define DETBOX_MAX_ALTERNATIVES 64  /* largest top_k of detbox_label_log_probs_forward */
+
+/* y = (x - mean) / sqrt(var + eps) * weight + bias over rows of D elements (var: the mean of the squared deviations).
+ *   weight, bias  [D] of param_dtype, each may be NULL
+ *   y [rows,D]; stats [rows,2] (mean, 1/sqrt(var + eps)) for the backward call, or NULL
+ * The backward call writes whichever of grad_x [rows,D], grad_weight [D], grad_bias [D] is not NULL. */
+int detbox_layer_norm_forward(int dtype, const void *x, int64_t ldx, int param_dtype, const void *weight, const void *bias,
+                              int64_t rows, int64_t D, float eps, void *y, float *stats, void *stream);
+size_t detbox_layer_norm_backward_workspace_bytes(int64_t rows, int64_t D);
+int detbox_layer_norm_backward(int dtype, const void *grad_y, int64_t ldg, const void *x, int64_t ldx, int param_dtype,
+                               const void *weight, const float *stats, int64_t rows, int64_t D,
+                               void *grad_x, void *grad_weight, void *grad_bias,
+                               void *workspace, size_t workspace_bytes, void *stream);
+
+/* y = act(x W^T + bias) + residual: x [M,K], weight [N,K], y [M,N], all but y of `dtype`; y and the residual [M,N] are of
+ * out_dtype (= dtype, or DETBOX_F32); bias [N] of bias_dtype or NULL; residual or NULL.
+ *   pre_activation [M,N] of `dtype` receives x W^T + bias for the backward call, or NULL
+ * The backward call takes grad_y of grad_dtype (= the forward call's out_dtype) and writes whichever of grad_x [M,K],
+ * grad_weight [N,K], grad_bias [N] is not NULL; the residual's gradient is grad_y itself.  pre_activation may be NULL
+ * with DETBOX_ACTIVATION_NONE, weight where grad_x is, x where grad_weight is. */
+size_t detbox_linear_workspace_bytes(int dtype, int64_t M, int64_t N, int64_t K);
+int detbox_linear_forward(int dtype, int activation, const void *x, int64_t ldx, const void *weight, int64_t ldw,
+                          int bias_dtype, const void *bias, const void *residual, int64_t ldr,
+                          int64_t M, int64_t N, int64_t K, int out_dtype, void *y, void *pre_activation,
+                          void *workspace, size_t workspace_bytes, void *stream);
+size_t detbox_linear_backward_workspace_bytes(int dtype, int activation, int grad_dtype, int64_t M, int64_t N, int64_t K);
+int detbox_linear_backward(int dtype, int activation, int grad_dtype, const void *grad_y, int64_t ldg,
+                           const void *pre_activation, const void *x, int64_t ldx, const void *weight, int64_t ldw,
+                           int64_t M, int64_t N, int64_t K, void *grad_x, void *grad_weight, int bias_dtype, void *grad_bias,
+                           void *workspace, size_t workspace_bytes, void *stream);
+
+/* Of every row of logits [rows,C]: the log probability of its label, the entropy of its distribution, its best
+ * alternatives.
+ *   labels        [rows]; a label outside [0, C) takes no part: log probability 0
+ *   log_probs     [rows]; entropy [rows] or NULL
+ *   top_log_probs, top_ids [rows,top_k]: the largest logits, the lower index first among equals, NaN above everything;
+ *                 0 <= top_k <= min(C, DETBOX_MAX_ALTERNATIVES)
+ *   stats         [rows,2] (largest logit, sum of exp(logit - largest)) for the backward call, or NULL
+ * A logit of -inf is a class that cannot be.  A row of -inf only has no distribution: log probability -inf, entropy 0,
+ * alternatives 0 .. top_k-1 at -inf, gradient 0.  A row that holds NaN or +inf gives NaN.
+ * The backward call writes grad_logits [rows,C] of `dtype` from the gradients of log_probs and entropy (each [rows], or
+ * NULL for none; grad_entropy needs the entropy of the forward call).  Rows that take no part in either get 0. */
+size_t detbox_label_log_probs_workspace_bytes(int64_t rows, int64_t C, int top_k);
+int detbox_label_log_probs_forward(int dtype, const void *logits, int64_t ld, const int64_t *labels, int64_t rows, int64_t C,
+                                   int top_k, float *log_probs, float *entropy, float *top_log_probs, int64_t *top_ids,
+                                   float *stats, void *workspace, size_t workspace_bytes, void *stream);
+int detbox_label_log_probs_backward(int dtype, const void *logits, int64_t ld, const int64_t *labels, int64_t rows, int64_t C,
+                                    const float *stats, const float *entropy, const float *grad_log_probs,
+                                    const float *grad_entropy, void *grad_logits, void *stream);
+
 /* ---- inference: activation + threshold + exact top-k + decode ---------------------------- */
 
 /* activations applied to the head output before the threshold */
@@ -280,7 +347,8 @@ int detbox_pack_detections_wire(const float *boxes, const float *scores, const i
  * "select_plan", "select_scan", "select_check", "score_hist", "select_kth",
  * "select_refine", "select_emit", "select_finalize", "select_direct_stats", "select_direct", "nms_segments", "nms_scan", "nms_merge",
  * "nms_split", "nms_tile", "pack_detections", "pack_wire", "topk_mask", "focal_forward", "focal_backward",
- * "smooth_l1_forward", "smooth_l1_backward". */
+ * "smooth_l1_forward", "smooth_l1_backward", "layer_norm_forward", "layer_norm_backward", "linear_forward",
+ * "linear_backward", "label_log_probs_forward", "label_log_probs_backward" (the last six: all launches of a call). */
 int detbox_profile_enable(int on);
 /* Restricts the timing to the one kernel called `name` (NULL or "" = every kernel again), so that a
  * timed run pays the event overhead for that kernel only. */

@@ -30,6 +30,17 @@ SIGNATURES = {
     'detbox_focal_loss_backward': (_i32, [_p, _p, _i64, _i64, _f32, _f32, _p, _p, _p]),
     'detbox_smooth_l1_masked_forward': (_i32, [_p, _p, _p, _i64, _p, _p]),
     'detbox_smooth_l1_masked_backward': (_i32, [_p, _p, _p, _i64, _p, _p, _p]),
+    'detbox_layer_norm_forward': (_i32, [_i32, _p, _i64, _i32, _p, _p, _i64, _i64, _f32, _p, _p, _p]),
+    'detbox_layer_norm_backward_workspace_bytes': (_sz, [_i64, _i64]),
+    'detbox_layer_norm_backward': (_i32, [_i32, _p, _i64, _p, _i64, _i32, _p, _p, _i64, _i64, _p, _p, _p, _p, _sz, _p]),
+    'detbox_linear_workspace_bytes': (_sz, [_i32, _i64, _i64, _i64]),
+    'detbox_linear_forward': (_i32, [_i32, _i32, _p, _i64, _p, _i64, _i32, _p, _p, _i64, _i64, _i64, _i64, _i32, _p, _p, _p, _sz, _p]),
+    'detbox_linear_backward_workspace_bytes': (_sz, [_i32, _i32, _i32, _i64, _i64, _i64]),
+    'detbox_linear_backward': (_i32, [_i32, _i32, _i32, _p, _i64, _p, _p, _i64, _p, _i64, _i64, _i64, _i64, _p, _p, _i32, _p,
+                                      _p, _sz, _p]),
+    'detbox_label_log_probs_workspace_bytes': (_sz, [_i64, _i64, _i32]),
+    'detbox_label_log_probs_forward': (_i32, [_i32, _p, _i64, _p, _i64, _i64, _i32, _p, _p, _p, _p, _p, _p, _sz, _p]),
+    'detbox_label_log_probs_backward': (_i32, [_i32, _p, _i64, _p, _i64, _i64, _p, _p, _p, _p, _p, _p]),
     'detbox_activate_scores': (_i32, [_i32, _p, _p, _i64, _i64, _i64, _p, _p]),
     'detbox_select_decode_workspace_bytes': (_sz, [_i64, _i64, _i64, _i32, _i32, _i32]),
     'detbox_select_decode': (_i32, [_i32, _i32, _p, _p, _p, _p, _i64, _i64, _i64, _i32, _i32, _f32, _i32, _f32,

@@ -23,4 +23,5 @@ def bind_boxops(model, name: str, **ctor):
     model.loss = impl.loss
     model.pre_predict = impl.pre_predict
     model.detect = impl.detect
+    model.head_logits = impl.head_logits
     return model

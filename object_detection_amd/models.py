@@ -16,7 +16,7 @@ without leaving the device.
 """
 from __future__ import annotations
 
-from typing import List, Sequence, Tuple
+from typing import List, Optional, Sequence, Tuple
 
 import torch
 import torch.nn.functional as F
@@ -53,6 +53,20 @@ class _BoxOps:
         return self._dev_tables[key]
 
     activation = ops.ACT_SOFTMAX
+
+    def head_logits(self, features: torch.Tensor, embeddings: torch.Tensor, bias: Optional[torch.Tensor] = None,
+                    tower: Sequence[tuple] = (), activation: str = 'relu') -> torch.Tensor:
+        """Class logits [B,P,C] in fp32 from one feature vector per anchor or point: the `out_confs` that loss, pre_predict
+        and detect take, for heads that score classes by embeddings (the reference's heads end in a convolution instead,
+        src/models/retinanet.py:100-106).  features [B,P,D], embeddings [C,D] with C = self.nc, bias [C];
+        tower: layers (norm_weight, norm_bias, weight, bias) with weight [D,D], each
+            features = activation(layer_norm(features) weight^T + bias) + features
+        Differentiable in everything but the choice of activation."""
+        if embeddings.shape[0] != self.nc:
+            raise ValueError(f'head_logits: {embeddings.shape[0]} class embeddings for {self.nc} classes')
+        for norm_weight, norm_bias, weight, b in tower:
+            features = ops.linear(ops.layer_norm(features, norm_weight, norm_bias), weight, b, activation, residual=features)
+        return ops.linear(features, embeddings, bias, out_dtype=torch.float32)
 
     # -- subclasses provide: _anchors_for_decode(), _head(outputs) -> (locs, class head output, extra)
     def _activate(self, outputs: tuple):
