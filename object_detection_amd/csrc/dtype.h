@@ -1,6 +1,7 @@
 // Element types of the class-head operators (norm.hip, linear.hip, logprob.hip): fp32, bfloat16 and fp16 in memory,
 // fp32 in registers.  Not part of the C ABI.
 #pragma once
+#include <type_traits>
 #include "detbox_internal.h"
 
 namespace detbox {
@@ -29,6 +30,91 @@ __device__ inline void store_from_float(void *p, int dtype, int64_t i, float v) 
     if (dtype == DETBOX_F32) static_cast<float *>(p)[i] = v;
     else if (dtype == DETBOX_BF16) static_cast<__bf16 *>(p)[i] = (__bf16)v;
     else static_cast<_Float16 *>(p)[i] = (_Float16)v;
+}
+
+// Sixteen bytes of elements from any address that is a multiple of the element's size: rows of odd length start anywhere, and
+// the memory pipeline takes a wide access at any such address.
+typedef uint32_t detbox_u4 __attribute__((ext_vector_type(4)));
+typedef uint32_t detbox_u4_at2 __attribute__((ext_vector_type(4), aligned(2), may_alias));
+typedef uint32_t detbox_u4_at4 __attribute__((ext_vector_type(4), aligned(4), may_alias));
+template <typename T> using raw_pack = std::conditional_t<sizeof(T) == 2, detbox_u4_at2, detbox_u4_at4>;
+template <typename T> constexpr int VEC_OF = 16 / (int)sizeof(T);
+template <typename T>
+__device__ inline void load_pack(float (&v)[VEC_OF<T>], const T *p) {
+    const detbox_u4 u = *reinterpret_cast<const raw_pack<T> *>(p);
+    if constexpr (sizeof(T) == 4) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) v[i] = __uint_as_float(u[i]);
+    } else {
+        typedef T t8 __attribute__((ext_vector_type(8)));
+        const t8 t = __builtin_bit_cast(t8, u);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) v[i] = (float)t[i];
+    }
+}
+template <typename T>
+__device__ inline void store_pack(T *p, const float (&v)[VEC_OF<T>]) {
+    detbox_u4 u;
+    if constexpr (sizeof(T) == 4) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) u[i] = __float_as_uint(v[i]);
+    } else {
+        typedef T t8 __attribute__((ext_vector_type(8)));
+        t8 t;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) t[i] = (T)v[i];
+        u = __builtin_bit_cast(detbox_u4, t);
+    }
+    *reinterpret_cast<raw_pack<T> *>(p) = u;
+}
+// The first n of a pack; the rest reads as `fill` and is not touched in memory.
+template <typename T>
+__device__ inline void load_pack(float (&v)[VEC_OF<T>], const T *p, int64_t n, float fill) {
+    if (n >= VEC_OF<T>) {
+        load_pack<T>(v, p);
+    } else {
+#pragma unroll
+        for (int i = 0; i < VEC_OF<T>; ++i) v[i] = i < n ? (float)p[i] : fill;
+    }
+}
+template <typename T>
+__device__ inline void store_pack(T *p, int64_t n, const float (&v)[VEC_OF<T>]) {
+    if (n >= VEC_OF<T>) {
+        store_pack<T>(p, v);
+    } else {
+#pragma unroll
+        for (int i = 0; i < VEC_OF<T>; ++i)
+            if (i < n) p[i] = (T)v[i];
+    }
+}
+
+// Sum and maximum over groups of G consecutive lanes, in every lane of the group.
+template <int G>
+__device__ inline float group_sum(float v) {
+    if constexpr (G > 1) v += lane_xor_f32<1>(v);
+    if constexpr (G > 2) v += lane_xor_f32<2>(v);
+    if constexpr (G > 4) v += lane_xor_f32<4>(v);
+    if constexpr (G > 8) v += lane_xor_f32<8>(v);
+    if constexpr (G > 16) v += lane_xor_f32<16>(v);
+    if constexpr (G > 32) v += lane_xor_f32<32>(v);
+    return v;
+}
+template <int G>
+__device__ inline float group_max(float v) {
+    if constexpr (G > 1) v = fmaxf(v, lane_xor_f32<1>(v));
+    if constexpr (G > 2) v = fmaxf(v, lane_xor_f32<2>(v));
+    if constexpr (G > 4) v = fmaxf(v, lane_xor_f32<4>(v));
+    if constexpr (G > 8) v = fmaxf(v, lane_xor_f32<8>(v));
+    if constexpr (G > 16) v = fmaxf(v, lane_xor_f32<16>(v));
+    if constexpr (G > 32) v = fmaxf(v, lane_xor_f32<32>(v));
+    return v;
+}
+template <int G>
+__device__ inline uint64_t group_max_u64(uint64_t v) {
+#define DETBOX_STEP(J) if constexpr (G > J) { const uint64_t o = lane_xor_u64<J>(v); v = o > v ? o : v; }
+    DETBOX_STEP(1) DETBOX_STEP(2) DETBOX_STEP(4) DETBOX_STEP(8) DETBOX_STEP(16) DETBOX_STEP(32)
+#undef DETBOX_STEP
+    return v;
 }
 
 __device__ inline float wave_sum(float v) {
