@@ -40,8 +40,12 @@ typedef uint32_t detbox_u4_at4 __attribute__((ext_vector_type(4), aligned(4), ma
 template <typename T> using raw_pack = std::conditional_t<sizeof(T) == 2, detbox_u4_at2, detbox_u4_at4>;
 template <typename T> constexpr int VEC_OF = 16 / (int)sizeof(T);
 template <typename T>
-__device__ inline void load_pack(float (&v)[VEC_OF<T>], const T *p) {
-    const detbox_u4 u = *reinterpret_cast<const raw_pack<T> *>(p);
+__device__ inline detbox_u4 load_raw(const T *p) { return *reinterpret_cast<const raw_pack<T> *>(p); }
+// The same for data that is not read again soon: it does not displace what is.
+template <typename T>
+__device__ inline detbox_u4 load_raw_nt(const T *p) { return __builtin_nontemporal_load(reinterpret_cast<const raw_pack<T> *>(p)); }
+template <typename T>
+__device__ inline void unpack(float (&v)[VEC_OF<T>], const detbox_u4 u) {
     if constexpr (sizeof(T) == 4) {
 #pragma unroll
         for (int i = 0; i < 4; ++i) v[i] = __uint_as_float(u[i]);
@@ -66,6 +70,33 @@ __device__ inline void store_pack(T *p, const float (&v)[VEC_OF<T>]) {
         u = __builtin_bit_cast(detbox_u4, t);
     }
     *reinterpret_cast<raw_pack<T> *>(p) = u;
+}
+template <typename T>
+__device__ inline void load_pack(float (&v)[VEC_OF<T>], const T *p) { unpack<T>(v, load_raw<T>(p)); }
+// Packs u = 0 .. U-1 of a row of C >= VEC elements at c + u * step, any of them partly or wholly behind its end (those read as
+// `fill`).  All U loads are issued before the first is looked at; the address of one that would pass the end is moved back.
+template <typename T, int U>
+__device__ inline void load_packs_to_end(float (&v)[U][VEC_OF<T>], const T *row, int64_t c, int64_t step, int64_t C, float fill) {
+    constexpr int VEC = VEC_OF<T>;
+    detbox_u4 raw[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u) raw[u] = load_raw<T>(row + (c + u * step + VEC <= C ? c + u * step : C - VEC));
+#pragma unroll
+    for (int u = 0; u < U; ++u) unpack<T>(v[u], raw[u]);
+#pragma unroll
+    for (int u = 0; u < U; ++u)
+        if (c + u * step + VEC > C) {
+            // what was loaded are the row's last VEC elements: the wanted ones move down, the fill moves in
+            const int64_t by = c + u * step + VEC - C;
+#pragma unroll
+            for (int b = VEC / 2; b > 0; b >>= 1)
+#pragma unroll
+                for (int i = 0; i < VEC; ++i) v[u][i] = (by & b) ? (i + b < VEC ? v[u][i + b < VEC ? i + b : 0] : fill) : v[u][i];
+            if (by >= VEC) {
+#pragma unroll
+                for (int i = 0; i < VEC; ++i) v[u][i] = fill;
+            }
+        }
 }
 // The first n of a pack; the rest reads as `fill` and is not touched in memory.
 template <typename T>

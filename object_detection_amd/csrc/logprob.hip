@@ -125,34 +125,37 @@ __global__ __launch_bounds__(LP_BLOCK) void logprob_rows_kernel(const T *__restr
 
 // Best words of one wave's share of a row: a buffer in LDS that takes every logit above `bar`, and is cut to the top_k best
 // when the next step might not fit.  The bar then is the value of the last one kept: the wave walks its share in index
-// order, so a later equal value is not better.
+// order, so a later equal value is not better.  The first bar is the top_k-th largest of the 64 lanes' maxima over the wave's
+// first round, which top_k logits of that round reach: on ordinary logits little more than top_k words are ever taken and
+// nothing is cut (2048 rows of 49999, five alternatives: 157 us with a buffer that is filled by the first step and cut, 72 us
+// so).
 constexpr int BUF = 640;
 
 struct WaveBest {
     uint64_t *buf;
     int count;
-    float bar;              // NaN: everything is taken
+    float bar;              // -inf at first: a class that cannot be is never among the words
 };
 
-// Keeps the k largest of count <= BUF distinct words.  T grows bit by bit to the largest prefix that k words reach.
-__device__ inline void cut_best(WaveBest &b, int k) {
+// Keeps the k largest of count <= 64 * N distinct words.  T grows bit by bit to the largest prefix that k words reach.
+template <int N>
+__device__ inline void cut_words(WaveBest &b, int k) {
     const int lane = threadIdx.x & 63;
-    if (b.count <= k) return;
-    uint64_t w[BUF / 64];
+    uint64_t w[N];
 #pragma unroll
-    for (int i = 0; i < BUF / 64; ++i) w[i] = i * 64 + lane < b.count ? b.buf[i * 64 + lane] : 0;
+    for (int i = 0; i < N; ++i) w[i] = i * 64 + lane < b.count ? b.buf[i * 64 + lane] : 0;
     uint64_t T = 0;
     for (int bit = 63; bit >= 0; --bit) {
         const uint64_t c = T | (1ull << bit);
         int n = 0;
 #pragma unroll
-        for (int i = 0; i < BUF / 64; ++i) n += __popcll(__ballot(w[i] >= c));
+        for (int i = 0; i < N; ++i) n += __popcll(__ballot(w[i] >= c));
         if (n >= k) T = c;
         if (n == k) break;
     }
     int at = 0;
 #pragma unroll
-    for (int i = 0; i < BUF / 64; ++i) {
+    for (int i = 0; i < N; ++i) {
         const bool keep = w[i] >= T && w[i] != 0;
         const unsigned long long mask = __ballot(keep);
         if (keep) b.buf[at + __popcll(mask & ((1ull << lane) - 1))] = w[i];
@@ -161,6 +164,27 @@ __device__ inline void cut_best(WaveBest &b, int k) {
     b.count = at;
     b.bar = __uint_as_float(bits_from_okey((uint32_t)(T >> 32)));
     __builtin_amdgcn_wave_barrier();
+}
+__device__ inline void cut_best(WaveBest &b, int k) {
+    if (b.count <= k) return;
+    if (b.count <= 192) cut_words<3>(b, k);
+    else cut_words<BUF / 64>(b, k);
+}
+
+// The largest T that k lanes' keys reach (0 where fewer than k lanes have one).
+__device__ inline uint32_t kth_key(uint32_t key, int k) {
+    uint32_t T = 0;
+    for (int bit = 31; bit >= 0; --bit) {
+        const uint32_t c = T | (1u << bit);
+        const int n = __popcll(__ballot(key >= c));
+        if (n >= k) T = c;
+        if (n == k) break;
+    }
+    return T;
+}
+// A bar that every value of at least T's passes (no key lies between those of the negative numbers and +0).
+__device__ inline float bar_below(uint32_t T) {
+    return __uint_as_float(bits_from_okey(T == 0x80000000u ? 0x7ffffffeu : T - 1u));
 }
 
 __device__ inline void offer(WaveBest &b, bool take, uint64_t word) {
@@ -172,29 +196,54 @@ __device__ inline void offer(WaveBest &b, bool take, uint64_t word) {
 // The workgroup's best of its waves' buffers: words[0 .. n) in LDS, n <= LP_WAVES * 64; rank of a word = how many are larger.
 __device__ inline int join_waves(WaveBest &b, int k, uint64_t *words, int *counts) {
     const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
-    cut_best(b, k);
+    if (b.count > DETBOX_MAX_ALTERNATIVES) cut_best(b, k);
     if (lane == 0) counts[w] = b.count;
     __syncthreads();
     int at = 0, n = 0;
     for (int i = 0; i < LP_WAVES; ++i) { if (i < w) at += counts[i]; n += counts[i]; }
-    const uint64_t mine = lane < b.count ? b.buf[lane] : 0;
-    if (lane < b.count) words[at + lane] = mine;
+    if (lane < b.count) words[at + lane] = b.buf[lane];
+    if (threadIdx.x < 8) words[n + threadIdx.x] = 0;                       // rank_of reads in eights
     __syncthreads();
     return n;
 }
+constexpr int WORDS = LP_WAVES * DETBOX_MAX_ALTERNATIVES + 8;
 __device__ inline int rank_of(uint64_t word, const uint64_t *words, int n) {
     int r = 0;
-    for (int i = 0; i < n; ++i) r += words[i] > word;
+    for (int i = 0; i < n; i += 8)
+#pragma unroll
+        for (int j = 0; j < 8; ++j) r += words[i + j] > word;
     return r;
+}
+
+// Writes a row's alternatives from the n words of its workgroup (more than top_k of them, or all of the row's logits above
+// -inf).  What is missing to top_k are classes at -inf: the lowest indices that are no word's.
+template <typename T>
+__device__ inline void write_alternatives(const Outputs &o, const T *xr, int64_t row, int top_k, const uint64_t *words, int n, float m, float s) {
+    if (threadIdx.x < n) {
+        const uint64_t w = words[threadIdx.x];
+        const int r = rank_of(w, words, n);
+        if (r < top_k) write_alternative(o, xr, row, top_k, r, w, m, s);
+    }
+    if (n < top_k && threadIdx.x < top_k) {
+        const uint32_t i = threadIdx.x;
+        int below = 0;
+        bool taken = false;
+        for (int j = 0; j < n; ++j) {
+            const uint32_t at = ~(uint32_t)words[j];
+            below += at < i;
+            taken |= at == i;
+        }
+        const int r = n + (int)i - below;
+        if (!taken && r < top_k) write_alternative(o, xr, row, top_k, r, (uint64_t)(uint32_t)~i, m, s);
+    }
 }
 
 // Block-wide merge of every lane's running sums into (m, s, t) of all threads.
 __device__ inline void block_sums(float &m, float &s, float &t, float *sm, float *ss, float *st) {
-#pragma unroll
-    for (int o = 1; o < 64; o <<= 1) {
-        const float m2 = __shfl_xor(m, o), s2 = __shfl_xor(s, o), t2 = __shfl_xor(t, o);
-        merge_sums(m, s, t, m2, s2, t2);
-    }
+    const float most = group_max<64>(m);
+    merge_sums(m, s, t, most, 0.f, 0.f);                                   // to the wave's reference
+    s = group_sum<64>(s);
+    t = group_sum<64>(t);
     const int w = threadIdx.x >> 6;
     if ((threadIdx.x & 63) == 0) { sm[w] = m; ss[w] = s; st[w] = t; }
     __syncthreads();
@@ -224,6 +273,13 @@ __device__ void slow_alternatives(const Outputs &o, const T *xr, int64_t row, in
     }
 }
 
+// Elements in front of the row's first cache line of 128 bytes (at most 63: one per lane of a wave).
+template <typename T>
+__device__ inline int head_of(const T *xr, int64_t C) {
+    const int h = (int)((0 - (uintptr_t)xr) % 128 / sizeof(T));
+    return h < C ? h : (int)C;
+}
+
 struct Partial { float m, s, t, unused; };
 
 // One workgroup per (row, piece).  pieces == 1: the row's results are written here; otherwise a Partial and, with TOP, top_k
@@ -236,7 +292,7 @@ __global__ __launch_bounds__(LP_BLOCK) void logprob_long_kernel(const T *__restr
     constexpr int VEC = VEC_OF<T>, U = 4, STEP = 64 * VEC;
     static_assert(STEP + DETBOX_MAX_ALTERNATIVES <= BUF, "a step must fit the buffer");
     __shared__ uint64_t s_buf[TOP ? LP_WAVES * BUF : 1];
-    __shared__ uint64_t s_words[LP_WAVES * DETBOX_MAX_ALTERNATIVES];
+    __shared__ uint64_t s_words[WORDS];
     __shared__ float s_m[LP_WAVES], s_s[LP_WAVES], s_t[LP_WAVES];
     __shared__ int s_n[LP_WAVES];
     const int lane = threadIdx.x & 63, wv = threadIdx.x >> 6;
@@ -245,7 +301,7 @@ __global__ __launch_bounds__(LP_BLOCK) void logprob_long_kernel(const T *__restr
         const int64_t row = job / pieces, lo = (job % pieces) * piece, hi = lo + piece < C ? lo + piece : C;
         const T *xr = x + row * ld;
         float m = -INFINITY, s = 0.f, t = 0.f;
-        WaveBest best{s_buf + (TOP ? wv * BUF : 0), 0, __builtin_nanf("")};
+        WaveBest best{s_buf + (TOP ? wv * BUF : 0), 0, -INFINITY};
 
         auto take_in = [&](const float (&v)[VEC]) {
             float top = v[0];
@@ -266,33 +322,69 @@ __global__ __launch_bounds__(LP_BLOCK) void logprob_long_kernel(const T *__restr
             }
             return top;
         };
-        auto alternatives = [&](const float (&v)[VEC], float top, int64_t c, int64_t end) {
+        // left: how many of the pack's logits are there
+        auto alternatives = [&](const float (&v)[VEC], float top, int64_t c, int left) {
             if (!__any(!(top <= best.bar))) return;
             if (best.count + STEP > BUF) cut_best(best, top_k);
-            for (int i = 0; i < VEC; ++i)                                  // not in index order inside the step: words are distinct
-                offer(best, c + i < end && !(v[i] <= best.bar), rank_word(v[i], (uint32_t)(c + i)));
-            if (best.bar != best.bar) cut_best(best, top_k);               // the first step sets the bar
+#pragma unroll
+            for (int i = 0; i < VEC; ++i) {                                // not in index order inside the step: words are distinct
+                const bool take = i < left && !(v[i] <= best.bar);
+                if (__any(take)) offer(best, take, rank_word(v[i], (uint32_t)(c + i)));
+            }
         };
 
-        int64_t c = lo + (int64_t)wv * STEP * U + lane * VEC;
-        for (; c - lane * VEC + STEP * U <= hi; c += (int64_t)LP_WAVES * STEP * U) {
-            float v[U][VEC];
+        // Steps start at cache lines: rows that start off them cost a fifth of the bandwidth (4096 rows of bf16: 131072 logits
+        // 186 us, 131071 logits 229 us before, 182 so); the row's first few logits go one per lane of the first wave.  Loads
+        // are not kept in the caches: 1.07 GB 163 us against 182; at 268 MB, where the backward pass might have found some of
+        // them, forward + backward are 47 + 81 us against 79 + 78, at 134 MB 26 + 43 against 28 + 41.
+        const int head = head_of<T>(xr, C);
+        if (lo == 0 && head && wv == 0) {
+            float v[VEC];
 #pragma unroll
-            for (int u = 0; u < U; ++u) load_pack<T>(v[u], xr + c + u * STEP);
-#pragma unroll
-            for (int u = 0; u < U; ++u) {
-                const float top = take_in(v[u]);
-                if (TOP) alternatives(v[u], top, c + u * STEP, hi);
-            }
+            for (int i = 0; i < VEC; ++i) v[i] = -INFINITY;
+            if (lane < head) v[0] = (float)xr[lane];
+            const float top = take_in(v);
+            if (TOP) alternatives(v, top, lane, lane < head);
         }
-        if (c - lane * VEC < hi) {                                         // the wave's last, partial round
-            for (int u = 0; u < U; ++u) {
-                const int64_t cu = c + u * STEP;
-                float v[VEC];
-                load_pack<T>(v, xr + cu, hi - cu, -INFINITY);
-                const float top = take_in(v);
-                if (TOP) alternatives(v, top, cu, hi);
+        const int64_t first = lo + head, end = hi + head < C ? hi + head : C;
+        bool fresh = true;
+        auto round = [&](const float (&v)[U][VEC], int64_t c, auto whole) {
+            constexpr bool WHOLE = decltype(whole)::value;                 // all of the round's logits are there
+            float tops[U];
+#pragma unroll
+            for (int u = 0; u < U; ++u) tops[u] = take_in(v[u]);
+            if (!TOP) return;
+            uint32_t reach = 0;
+            if (fresh) {
+                float most = tops[0];
+#pragma unroll
+                for (int u = 1; u < U; ++u) most = fmaxf(most, tops[u]);
+                reach = kth_key(WHOLE || c < end ? okey_from_bits(__float_as_uint(most)) : 0u, top_k);
+                if (reach > 0x007fffffu) best.bar = bar_below(reach);     // 0x007fffff: the key of -inf
             }
+#pragma unroll
+            for (int u = 0; u < U; ++u) {
+                const int64_t left = end - c - u * STEP;
+                alternatives(v[u], tops[u], c + u * STEP, WHOLE || left >= VEC ? VEC : left < 0 ? 0 : (int)left);
+            }
+            const float at = __uint_as_float(bits_from_okey(reach));
+            if (fresh && reach > 0x007fffffu && !(at < best.bar)) best.bar = at;
+            fresh = false;
+        };
+        int64_t c = first + (int64_t)wv * STEP * U + lane * VEC;
+        for (; c - lane * VEC + STEP * U <= end; c += (int64_t)LP_WAVES * STEP * U) {
+            float v[U][VEC];
+            detbox_u4 raw[U];
+#pragma unroll
+            for (int u = 0; u < U; ++u) raw[u] = load_raw_nt<T>(xr + c + u * STEP);
+#pragma unroll
+            for (int u = 0; u < U; ++u) unpack<T>(v[u], raw[u]);
+            round(v, c, std::true_type{});
+        }
+        if (c - lane * VEC < end) {                                        // the wave's last, partial round
+            float v[U][VEC];
+            load_packs_to_end<T, U>(v, xr, c, STEP, end, -INFINITY);
+            round(v, c, std::false_type{});
         }
         block_sums(m, s, t, s_m, s_s, s_t);
         int n = 0;
@@ -307,10 +399,8 @@ __global__ __launch_bounds__(LP_BLOCK) void logprob_long_kernel(const T *__restr
                 if (s != s) {
                     __syncthreads();
                     slow_alternatives<T>(o, xr, row, C, top_k, m, s, s_words);
-                } else if (threadIdx.x < n) {
-                    const uint64_t w = s_words[threadIdx.x];
-                    const int r = rank_of(w, s_words, n);
-                    if (r < top_k) write_alternative(o, xr, row, top_k, r, w, m, s);
+                } else {
+                    write_alternatives<T>(o, xr, row, top_k, s_words, n, m, s);
                 }
             }
         } else {
@@ -332,7 +422,7 @@ __global__ __launch_bounds__(LP_BLOCK) void logprob_join_kernel(const T *__restr
                                                                 int64_t rows, int64_t C, int top_k, int pieces,
                                                                 const Partial *__restrict__ partial,
                                                                 const uint64_t *__restrict__ partial_words, Outputs o) {
-    __shared__ uint64_t s_buf[LP_WAVES * BUF], s_words[LP_WAVES * DETBOX_MAX_ALTERNATIVES];
+    __shared__ uint64_t s_buf[LP_WAVES * BUF], s_words[WORDS];
     __shared__ float s_m[LP_WAVES], s_s[LP_WAVES], s_t[LP_WAVES];
     __shared__ int s_n[LP_WAVES];
     const int wv = threadIdx.x >> 6;
@@ -353,7 +443,7 @@ __global__ __launch_bounds__(LP_BLOCK) void logprob_join_kernel(const T *__restr
             if (s != s) {
                 slow_alternatives<T>(o, xr, row, C, top_k, m, s, s_words);
             } else {
-                WaveBest best{s_buf + wv * BUF, 0, 0.f};
+                WaveBest best{s_buf + wv * BUF, 0, -INFINITY};
                 const int total = pieces * top_k;
                 for (int i0 = wv * 64; i0 < total; i0 += LP_BLOCK) {
                     const int i = i0 + (threadIdx.x & 63);
@@ -362,11 +452,7 @@ __global__ __launch_bounds__(LP_BLOCK) void logprob_join_kernel(const T *__restr
                     offer(best, w != 0, w);
                 }
                 const int n = join_waves(best, top_k, s_words, s_n);
-                if (threadIdx.x < n) {
-                    const uint64_t w = s_words[threadIdx.x];
-                    const int r = rank_of(w, s_words, n);
-                    if (r < top_k) write_alternative(o, xr, row, top_k, r, w, m, s);
-                }
+                write_alternatives<T>(o, xr, row, top_k, s_words, n, m, s);
             }
         }
         __syncthreads();
@@ -446,23 +532,33 @@ __global__ __launch_bounds__(LP_BLOCK) void logprob_long_grad_kernel(const T *__
         const RowGrad r = row_grad(row, C, labels, stats, entropy, grad_lp, grad_ent);
         const T *xr = x + row * ld;
         T *gr = gx + row * C;
-        if (lo + LP_BLOCK * VEC * U <= C) {
+        const int head = head_of<T>(gr, C);                 // the logits start where the gradient does unless they are strided
+        const bool at_head = lo == 0 && threadIdx.x < head;
+        float front[1] = {at_head ? (float)xr[threadIdx.x] : 0.f};
+        const int64_t first = lo + head;
+        if (first + LP_BLOCK * VEC * U <= C) {
             float v[U][VEC];
 #pragma unroll
-            for (int u = 0; u < U; ++u) load_pack<T>(v[u], xr + lo + (u * LP_BLOCK + threadIdx.x) * VEC);
+            for (int u = 0; u < U; ++u) unpack<T>(v[u], load_raw_nt<T>(xr + first + (u * LP_BLOCK + threadIdx.x) * VEC));
 #pragma unroll
             for (int u = 0; u < U; ++u) {
-                const int64_t c = lo + (u * LP_BLOCK + threadIdx.x) * VEC;
+                const int64_t c = first + (u * LP_BLOCK + threadIdx.x) * VEC;
                 grad_pack<VEC>(v[u], r, c);
                 store_pack<T>(gr + c, v[u]);
             }
         } else {
-            for (int64_t c = lo + threadIdx.x * VEC; c < C; c += LP_BLOCK * VEC) {
-                float v[VEC];
-                load_pack<T>(v, xr + c, C - c, -INFINITY);
-                grad_pack<VEC>(v, r, c);
-                store_pack<T>(gr + c, C - c, v);
+            float v[U][VEC];
+            load_packs_to_end<T, U>(v, xr, first + threadIdx.x * VEC, LP_BLOCK * VEC, C, -INFINITY);
+#pragma unroll
+            for (int u = 0; u < U; ++u) {
+                const int64_t c = first + (u * LP_BLOCK + threadIdx.x) * VEC;
+                grad_pack<VEC>(v[u], r, c);
+                store_pack<T>(gr + c, C - c, v[u]);
             }
+        }
+        if (at_head) {
+            grad_pack<1>(front, r, threadIdx.x);
+            gr[threadIdx.x] = (T)front[0];
         }
     }
 }
@@ -547,14 +643,12 @@ extern "C" int detbox_label_log_probs_forward(int dtype, const void *logits, int
                 words = ws.take<uint64_t>((size_t)rows * cut.pieces * top_k);
             }
             const dim3 grid(grid_of(rows * cut.pieces)), block(LP_BLOCK);
-            if (top_k && entropy)
-                logprob_long_kernel<T, true, true><<<grid, block, 0, s>>>(x, ld, labels, rows, C, top_k, cut.pieces, cut.piece, o, partial, words);
-            else if (top_k)
-                logprob_long_kernel<T, true, false><<<grid, block, 0, s>>>(x, ld, labels, rows, C, top_k, cut.pieces, cut.piece, o, partial, words);
-            else if (entropy)
-                logprob_long_kernel<T, false, true><<<grid, block, 0, s>>>(x, ld, labels, rows, C, top_k, cut.pieces, cut.piece, o, partial, words);
-            else
-                logprob_long_kernel<T, false, false><<<grid, block, 0, s>>>(x, ld, labels, rows, C, top_k, cut.pieces, cut.piece, o, partial, words);
+            auto launch = [&](auto top, auto ent) {
+                logprob_long_kernel<T, decltype(top)::value, decltype(ent)::value>
+                    <<<grid, block, 0, s>>>(x, ld, labels, rows, C, top_k, cut.pieces, cut.piece, o, partial, words);
+            };
+            if (top_k) entropy ? launch(std::true_type{}, std::true_type{}) : launch(std::true_type{}, std::false_type{});
+            else entropy ? launch(std::false_type{}, std::true_type{}) : launch(std::false_type{}, std::false_type{});
             if (cut.pieces > 1)
                 logprob_join_kernel<T><<<dim3(grid_of(rows)), block, 0, s>>>(x, ld, labels, rows, C, top_k, cut.pieces, partial, words, o);
         }
