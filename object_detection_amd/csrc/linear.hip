@@ -4,18 +4,43 @@
 // Products are summed in fp32.  What is rounded to the type of x before it is multiplied: dz (when g is wider than x or
 // there is an activation) and the z that the derivative is taken at; both are operands of the same matrix instructions as
 // x and W, which have that type.
+//
+// One tile kernel serves all three products.  Each operand lies in memory either along the contraction (x, W forward) or
+// across it (W in grad_x; dz and x in grad_W); both come into LDS as they lie, 16 bytes at a time, and only the read of a
+// fragment differs: a plain 16-byte read, or the transposing LDS read of 16-bit elements.
 #include "dtype.h"
 
 using namespace detbox;
 
 namespace {
 
-__device__ inline float sigmoid_f(float z) { return 1.0f / (1.0f + expf(-z)); }
+typedef float f32x4 __attribute__((ext_vector_type(4)));
+typedef short s16x4 __attribute__((ext_vector_type(4)));
+typedef __attribute__((address_space(3))) s16x4 lds_s16x4;
+typedef const void __attribute__((address_space(1))) *gptr_t;
+typedef void __attribute__((address_space(3))) *lptr_t;
+
+constexpr float LOG2E = 1.44269504088896340736f;
+__device__ inline float fast_exp(float d) { return __builtin_amdgcn_exp2f(d * LOG2E); }
+__device__ inline float sigmoid_f(float z) { return __builtin_amdgcn_rcpf(1.0f + fast_exp(-z)); }
+
+// Normal distribution function by Abramowitz and Stegun, Handbook of Mathematical Functions, 7.1.26 (error below 1.5e-7 / 2);
+// e is exp(-z^2 / 2), which the slope needs as well.
+__device__ inline float normal_cdf(float z, float e) {
+    const float u = fabsf(z) * 0.70710678118654752f;
+    const float t = __builtin_amdgcn_rcpf(fmaf(0.3275911f, u, 1.0f));
+    float q = fmaf(1.061405429f, t, -1.453152027f);
+    q = fmaf(q, t, 1.421413741f);
+    q = fmaf(q, t, -0.284496736f);
+    q = fmaf(q, t, 0.254829592f);
+    const float tail = 0.5f * q * t * e;
+    return z < 0.f ? tail : 1.0f - tail;
+}
 
 __device__ inline float act_value(float z, int act) {
     switch (act) {
         case DETBOX_ACTIVATION_RELU: return z > 0.f ? z : (z != z ? z : 0.f);
-        case DETBOX_ACTIVATION_GELU: return z < -1e4f ? 0.f : 0.5f * z * (1.0f + erff(z * 0.70710678118654752f));
+        case DETBOX_ACTIVATION_GELU: return z < -1e4f ? 0.f : z * normal_cdf(z, fast_exp(-0.5f * z * z));
         case DETBOX_ACTIVATION_SILU: return z < -1e4f ? 0.f : z * sigmoid_f(z);
         case DETBOX_ACTIVATION_SIGMOID: return sigmoid_f(z);
     }
@@ -26,8 +51,10 @@ __device__ inline float act_value(float z, int act) {
 __device__ inline float act_slope(float z, int act) {
     if (act == DETBOX_ACTIVATION_RELU) return z > 0.f ? 1.f : (z != z ? z : 0.f);
     z = z > 1e4f ? 1e4f : (z < -1e4f ? -1e4f : z);
-    if (act == DETBOX_ACTIVATION_GELU)
-        return 0.5f * (1.0f + erff(z * 0.70710678118654752f)) + z * 0.39894228040143268f * expf(-0.5f * z * z);
+    if (act == DETBOX_ACTIVATION_GELU) {
+        const float e = fast_exp(-0.5f * z * z);
+        return fmaf(z * 0.39894228040143268f, e, normal_cdf(z, e));
+    }
     if (act == DETBOX_ACTIVATION_SILU) { const float p = sigmoid_f(z); return p * (1.0f + z * (1.0f - p)); }
     if (act == DETBOX_ACTIVATION_SIGMOID) { const float p = sigmoid_f(z); return p * (1.0f - p); }
     return 1.f;
@@ -37,90 +64,413 @@ struct Epilogue {
     const void *bias; int bias_dtype;
     const void *residual; int64_t ldr;      // element type of the output
     int act;
-    void *pre;                              // z in the type of x, or null
-    int out_dtype;
+    void *pre; int pre_dtype;               // z, or null
+    void *out; int out_dtype;
 };
 
-constexpr int TILE = 64, TILE_K = 16;
-
-// C[m,n] = sum_k A[m * am + k * ak] * B[n * bn + k * bk]: every layout through element loads and fp32 arithmetic
-template <typename T>
-__global__ __launch_bounds__(256) void gemm_any_kernel(const T *__restrict__ A, int64_t am, int64_t ak, const T *__restrict__ B,
-                                                       int64_t bn, int64_t bk, int64_t M, int64_t N, int64_t K, Epilogue ep,
-                                                       void *C, int64_t tiles_n, int64_t tiles) {
-    __shared__ float sa[TILE_K][TILE + 4], sb[TILE_K][TILE + 4];
-    const int tx = threadIdx.x & 15, ty = threadIdx.x >> 4;
-    for (int64_t tile = blockIdx.x; tile < tiles; tile += gridDim.x) {
-        const int64_t m0 = tile / tiles_n * TILE, n0 = tile % tiles_n * TILE;
-        float acc[4][4] = {};
-        for (int64_t k0 = 0; k0 < K; k0 += TILE_K) {
-            __syncthreads();
-            for (int e = threadIdx.x; e < TILE * TILE_K; e += 256) {
-                const int k = ak == 1 ? e % TILE_K : e / TILE, m = ak == 1 ? e / TILE_K : e % TILE;
-                sa[k][m] = m0 + m < M && k0 + k < K ? (float)A[(m0 + m) * am + (k0 + k) * ak] : 0.f;
-            }
-            for (int e = threadIdx.x; e < TILE * TILE_K; e += 256) {
-                const int k = bk == 1 ? e % TILE_K : e / TILE, n = bk == 1 ? e / TILE_K : e % TILE;
-                sb[k][n] = n0 + n < N && k0 + k < K ? (float)B[(n0 + n) * bn + (k0 + k) * bk] : 0.f;
-            }
-            __syncthreads();
+// n <= 4 consecutive elements of a buffer whose type is known at run time, from any address of an element
+typedef uint32_t detbox_u2_at2 __attribute__((ext_vector_type(2), aligned(2), may_alias));
+__device__ inline f32x4 load4(const void *p, int dtype, int64_t i, int n) {
+    f32x4 v = {0.f, 0.f, 0.f, 0.f};
+    if (n >= 4) {
+        if (dtype == DETBOX_F32) return __builtin_bit_cast(f32x4, load_raw<float>(static_cast<const float *>(p) + i));
+        const detbox_u2_at2 u = *reinterpret_cast<const detbox_u2_at2 *>(static_cast<const uint16_t *>(p) + i);
 #pragma unroll
-            for (int k = 0; k < TILE_K; ++k)
-#pragma unroll
-                for (int i = 0; i < 4; ++i)
-#pragma unroll
-                    for (int j = 0; j < 4; ++j) acc[i][j] = fmaf(sa[k][ty * 4 + i], sb[k][tx * 4 + j], acc[i][j]);
+        for (int j = 0; j < 4; ++j) {
+            const uint16_t h = (uint16_t)(u[j >> 1] >> (16 * (j & 1)));
+            v[j] = dtype == DETBOX_BF16 ? __uint_as_float((uint32_t)h << 16) : (float)__builtin_bit_cast(_Float16, h);
         }
-        for (int i = 0; i < 4; ++i)
-            for (int j = 0; j < 4; ++j) {
-                const int64_t m = m0 + ty * 4 + i, n = n0 + tx * 4 + j;
-                if (m >= M || n >= N) continue;
-                float z = acc[i][j];
-                if (ep.bias) z += load_as_float(ep.bias, ep.bias_dtype, n);
-                if (ep.pre) static_cast<T *>(ep.pre)[m * N + n] = (T)z;
-                z = act_value(z, ep.act);
-                if (ep.residual) z += load_as_float(ep.residual, ep.out_dtype, m * ep.ldr + n);
-                store_from_float(C, ep.out_dtype, m * N + n, z);
+        return v;
+    }
+    for (int j = 0; j < n; ++j) v[j] = load_as_float(p, dtype, i + j);
+    return v;
+}
+__device__ inline void store4(void *p, int dtype, int64_t i, int n, f32x4 v) {
+    if (n >= 4) {
+        if (dtype == DETBOX_F32) {
+            *reinterpret_cast<detbox_u4_at4 *>(static_cast<float *>(p) + i) = __builtin_bit_cast(detbox_u4, v);
+            return;
+        }
+        detbox_u2_at2 u;
+        if (dtype == DETBOX_BF16) {
+            typedef __bf16 b4 __attribute__((ext_vector_type(4)));
+            u = __builtin_bit_cast(detbox_u2_at2, __builtin_convertvector(v, b4));
+        } else {
+            typedef _Float16 h4 __attribute__((ext_vector_type(4)));
+            u = __builtin_bit_cast(detbox_u2_at2, __builtin_convertvector(v, h4));
+        }
+        *reinterpret_cast<detbox_u2_at2 *>(static_cast<uint16_t *>(p) + i) = u;
+        return;
+    }
+    for (int j = 0; j < n; ++j) store_from_float(p, dtype, i + j, v[j]);
+}
+
+// Four neighbouring sums of row m, columns n .. n + 3 (those below N), through the epilogue.
+__device__ inline void finish4(const Epilogue &ep, int64_t m, int64_t n, int64_t N, f32x4 z) {
+    const int left = N - n < 4 ? (int)(N - n) : 4;
+    if (left <= 0) return;
+    if (ep.bias) z += load4(ep.bias, ep.bias_dtype, n, left);
+    if (ep.pre) store4(ep.pre, ep.pre_dtype, m * N + n, left, z);
+    if (ep.act != DETBOX_ACTIVATION_NONE) {
+#pragma unroll
+        for (int j = 0; j < 4; ++j) z[j] = act_value(z[j], ep.act);
+    }
+    if (ep.residual) z += load4(ep.residual, ep.out_dtype, m * ep.ldr + n, left);
+    store4(ep.out, ep.out_dtype, m * N + n, left, z);
+}
+
+// ---- tile kernel ---------------------------------------------------------------------------------------------------------
+
+// An operand: `rows` rows of the output's axis, contraction length in GemmArgs.  ACROSS == false: element (r, k) at
+// p[r * ld + k]; ACROSS == true: at p[k * ld + r].  extent: how far the axis that lies in order may be read (to the end of a
+// padded row where what is behind the operand's own end is zero).
+template <typename T>
+struct Operand { const T *p; int64_t ld; int64_t rows, extent; };
+
+template <typename T>
+struct GemmArgs {
+    Operand<T> a, b;            // output rows m from a, columns n from b
+    int64_t K;
+    int tiles_m, tiles_n, splits;
+    int64_t steps_per_split;    // contraction steps of one piece
+    Epilogue ep;
+    float *part;                // [splits][M][N] where splits > 1
+};
+
+// A step of the contraction is 128 bytes per row: 64 elements of 16 bits or 32 of fp32, eight chunks of 16 bytes.
+template <typename T> constexpr int STEP_K = 128 / (int)sizeof(T);
+
+// Where the chunks of a step lie in LDS.  Along: chunk c of row r at slot c ^ (r & 7) of the row's 128 bytes, so that the 16
+// rows a fragment read touches spread over all banks.  Across: rows of the contraction, each ROWS elements in units of 16
+// (one fragment's width); unit u of row k at u ^ swizzle(k), which spreads the rows that one read touches.
+template <typename T>
+__device__ inline int across_swizzle(int k) {
+    return sizeof(T) == 2 ? (k & 3) | ((k >> 3) & 1) << 2 : (k >> 2) & 3;
+}
+
+// The chunks of one step that a thread brings in: idx = j * THREADS + tid is also the place in LDS.
+template <typename T, bool ACROSS, int ROWS, int THREADS, bool ALIGNED>
+struct Stager {
+    static constexpr int VEC = VEC_OF<T>, COUNT = ROWS * 8 / THREADS, PER_K = ROWS / VEC, PER_UNIT = 16 / VEC;
+    const T *src[COUNT];        // of the step that is fetched next
+    int at[COUNT];              // contraction index of the chunk inside a step
+    int left[COUNT];            // across: how many of the chunk's elements exist
+    int64_t step;               // elements from one step to the next
+
+    __device__ void init(const Operand<T> &o, int64_t row0, int64_t k0) {
+        const int tid = threadIdx.x;
+        step = ACROSS ? STEP_K<T> * o.ld : STEP_K<T>;
+#pragma unroll
+        for (int j = 0; j < COUNT; ++j) {
+            const int idx = j * THREADS + tid;
+            if (ACROSS) {
+                const int k = idx / PER_K, slot = idx % PER_K;
+                const int unit = (slot / PER_UNIT) ^ across_swizzle<T>(k);
+                int64_t r = row0 + unit * 16 + (slot % PER_UNIT) * VEC;
+                at[j] = k;
+                const int64_t n = o.extent - r;
+                left[j] = n >= VEC ? VEC : n < 0 ? 0 : (int)n;
+                if (ALIGNED && n < VEC) r = o.extent - VEC;            // rows that do not exist: any values
+                if (!ALIGNED && n <= 0) r = 0;
+                src[j] = o.p + (k0 + k) * o.ld + r;
+            } else {
+                const int r = idx >> 3, chunk = (idx & 7) ^ (r & 7);
+                int64_t row = row0 + r;
+                if (row >= o.rows) row = o.rows - 1;                      // rows that do not exist: any values
+                at[j] = chunk * VEC;
+                left[j] = VEC;
+                src[j] = o.p + row * o.ld + k0 + chunk * VEC;
             }
+        }
+    }
+    // Chunk j of the next step, which starts k_left elements before the contraction's end; zeros behind the end.
+    __device__ detbox_u4 load(int j, int64_t k_left) {
+        const T *p = src[j];
+        src[j] = p + step;
+        if (ALIGNED) {
+            if (k_left >= STEP_K<T>) return *reinterpret_cast<const detbox_u4 *>(p);
+            detbox_u4 z = {0, 0, 0, 0};
+            if (at[j] < k_left) z = *reinterpret_cast<const detbox_u4 *>(p);
+            return z;
+        }
+        int n = left[j];
+        if (ACROSS) n = at[j] < k_left ? n : 0;
+        else if (k_left - at[j] < VEC) n = k_left - at[j] < 0 ? 0 : (int)(k_left - at[j]);
+        if (n == VEC) return load_raw<T>(p);
+        T e[VEC];
+#pragma unroll
+        for (int i = 0; i < VEC; ++i) e[i] = i < n ? p[i] : (T)0.f;
+        detbox_u4 u;
+        __builtin_memcpy(&u, e, 16);
+        return u;
+    }
+};
+
+// Fragment of 16 rows and four chunks' worth of contraction: lane l has row l % 16, its elements k of quarter l / 16.
+template <typename T, bool ACROSS, int ROWS>
+__device__ inline detbox_u4 read_fragment(const char *lds, int row0, int ks) {
+    const int lane = threadIdx.x & 63, r = lane & 15, q = lane >> 4;
+    if (!ACROSS) {
+        const int row = row0 + r;
+        return *reinterpret_cast<const detbox_u4 *>(lds + (row * 8 + ((ks * 4 + q) ^ (row & 7))) * 16);
+    }
+    if constexpr (sizeof(T) == 2) {
+        detbox_u4 u;
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+            const int k = ks * 32 + q * 8 + h * 4 + (r >> 2);
+            const char *p = lds + k * (ROWS * 2) + (((row0 >> 4) ^ across_swizzle<T>(k)) * 32) + (r & 3) * 8;
+            const s16x4 v = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4 *)p);
+            typedef uint32_t u2 __attribute__((ext_vector_type(2)));
+            const u2 w = __builtin_bit_cast(u2, v);
+            u[2 * h] = w[0];
+            u[2 * h + 1] = w[1];
+        }
+        return u;
+    } else {
+        detbox_u4 u;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            const int k = ks * 16 + q * 4 + j;
+            u[j] = *reinterpret_cast<const uint32_t *>(lds + k * (ROWS * 4) + (((row0 >> 4) ^ across_swizzle<T>(k)) * 64) + r * 4);
+        }
+        return u;
     }
 }
 
-// dz = g * act'(pre) in the type of x, and partial column sums of the unrounded dz per row slice
+// acc[n = 4 (l / 16) + i][m = l % 16] += sum over the fragments' contraction
+template <typename T>
+__device__ inline f32x4 multiply(detbox_u4 n, detbox_u4 m, f32x4 acc) {
+    if constexpr (std::is_same_v<T, __bf16>) {
+        typedef __bf16 v8 __attribute__((ext_vector_type(8)));
+        return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(v8, n), __builtin_bit_cast(v8, m), acc, 0, 0, 0);
+    } else if constexpr (std::is_same_v<T, _Float16>) {
+        typedef _Float16 v8 __attribute__((ext_vector_type(8)));
+        return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(v8, n), __builtin_bit_cast(v8, m), acc, 0, 0, 0);
+    } else {
+        const f32x4 a = __builtin_bit_cast(f32x4, n), b = __builtin_bit_cast(f32x4, m);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) acc = __builtin_amdgcn_mfma_f32_16x16x4f32(a[j], b[j], acc, 0, 0, 0);
+        return acc;
+    }
+}
+
+// Workgroups are dealt to the eight XCDs in turn.  Every XCD gets a run of neighbouring tiles, walked in bands of eight tile
+// rows, so that the operands' panels are shared in its L2.
+__device__ inline void tile_of(int wg, int tiles_m, int tiles_n, int &tm, int &tn) {
+    const int total = tiles_m * tiles_n, per = total / 8, rest = total % 8;
+    const int x = wg & 7, i = wg >> 3;
+    const int t = x * per + (x < rest ? x : rest) + i;
+    const int band = t / (8 * tiles_n), rows = tiles_m - band * 8 < 8 ? tiles_m - band * 8 : 8;
+    const int in = t - band * 8 * tiles_n;
+    tm = band * 8 + in % rows;
+    tn = in / rows;
+}
+
+template <typename T, bool AX, bool BX, int BM, int BN, int WM, int WN, bool ALIGNED>
+__global__ __launch_bounds__((BM / WM) * (BN / WN) * 64) void gemm_kernel(GemmArgs<T> g) {
+    constexpr int THREADS = (BM / WM) * (BN / WN) * 64, FM = WM / 16, FN = WN / 16;
+    constexpr int A_BYTES = BM * 128, B_BYTES = BN * 128, PAD = 4;
+    extern __shared__ __attribute__((aligned(16))) char lds[];
+    const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
+    const int wm = (wave % (BM / WM)) * WM, wn = (wave / (BM / WM)) * WN;
+    int tm, tn;
+    tile_of(blockIdx.x, g.tiles_m, g.tiles_n, tm, tn);
+    const int64_t m0 = (int64_t)tm * BM, n0 = (int64_t)tn * BN;
+    const int split = blockIdx.y;
+    const int64_t s0 = split * g.steps_per_split, all = (g.K + STEP_K<T> - 1) / STEP_K<T>;
+    const int64_t steps = all - s0 < g.steps_per_split ? all - s0 : g.steps_per_split;
+
+    Stager<T, AX, BM, THREADS, ALIGNED> sa;
+    Stager<T, BX, BN, THREADS, ALIGNED> sb;
+    const int64_t k0 = s0 * STEP_K<T>;
+    sa.init(g.a, m0, k0);
+    sb.init(g.b, n0, k0);
+    detbox_u4 ra[sa.COUNT], rb[sb.COUNT];
+    auto fetch = [&](int64_t s) {
+        const int64_t k_left = g.K - k0 - s * STEP_K<T>;
+#pragma unroll
+        for (int j = 0; j < sa.COUNT; ++j) ra[j] = sa.load(j, k_left);
+#pragma unroll
+        for (int j = 0; j < sb.COUNT; ++j) rb[j] = sb.load(j, k_left);
+    };
+    auto put = [&](int buf) {
+        char *la = lds + buf * (A_BYTES + B_BYTES), *lb = la + A_BYTES;
+#pragma unroll
+        for (int j = 0; j < sa.COUNT; ++j) *reinterpret_cast<detbox_u4 *>(la + (j * THREADS + threadIdx.x) * 16) = ra[j];
+#pragma unroll
+        for (int j = 0; j < sb.COUNT; ++j) *reinterpret_cast<detbox_u4 *>(lb + (j * THREADS + threadIdx.x) * 16) = rb[j];
+    };
+
+    f32x4 acc[FM][FN];
+#pragma unroll
+    for (int i = 0; i < FM; ++i)
+#pragma unroll
+        for (int j = 0; j < FN; ++j) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
+
+    if (steps > 0) {
+        fetch(0);
+        put(0);
+    }
+    __syncthreads();
+    for (int64_t s = 0; s < steps; ++s) {
+        if (s + 1 < steps) fetch(s + 1);
+        const char *la = lds + (s & 1) * (A_BYTES + B_BYTES), *lb = la + A_BYTES;
+#pragma unroll
+        for (int ks = 0; ks < 2; ++ks) {
+            detbox_u4 fa[FM], fb[FN];
+#pragma unroll
+            for (int i = 0; i < FM; ++i) fa[i] = read_fragment<T, AX, BM>(la, wm + i * 16, ks);
+#pragma unroll
+            for (int j = 0; j < FN; ++j) fb[j] = read_fragment<T, BX, BN>(lb, wn + j * 16, ks);
+#pragma unroll
+            for (int i = 0; i < FM; ++i)
+#pragma unroll
+                for (int j = 0; j < FN; ++j) acc[i][j] = multiply<T>(fb[j], fa[i], acc[i][j]);
+        }
+        if (s + 1 < steps) put((s + 1) & 1);
+        __syncthreads();
+    }
+
+    // The sums go through LDS, 64 rows of the wave's part at a time, so that rows are written (and the residual read) in order.
+    constexpr int HALF = WM < 64 ? WM : 64, ROW = WN + PAD, LANES = WN / 4;
+    float *mine = reinterpret_cast<float *>(lds) + wave * (HALF * ROW);
+    const int64_t M = g.a.rows, N = g.b.rows;
+#pragma unroll
+    for (int h = 0; h < WM / HALF; ++h) {
+        if (h) __builtin_amdgcn_wave_barrier();
+#pragma unroll
+        for (int i = 0; i < HALF / 16; ++i)
+#pragma unroll
+            for (int j = 0; j < FN; ++j)
+                *reinterpret_cast<f32x4 *>(mine + (i * 16 + (lane & 15)) * ROW + j * 16 + (lane >> 4) * 4) = acc[h * (HALF / 16) + i][j];
+        __builtin_amdgcn_wave_barrier();
+        for (int r = lane / LANES; r < HALF; r += 64 / LANES) {
+            const int64_t m = m0 + wm + h * HALF + r, n = n0 + wn + (lane % LANES) * 4;
+            if (m >= M) break;
+            const f32x4 z = *reinterpret_cast<const f32x4 *>(mine + r * ROW + (lane % LANES) * 4);
+            if (g.splits == 1) finish4(g.ep, m, n, N, z);
+            else if (n < N) store4(g.part, DETBOX_F32, ((int64_t)split * M + m) * N + n, N - n < 4 ? (int)(N - n) : 4, z);
+        }
+    }
+}
+
+// Adds the pieces of the contraction in order and applies the epilogue.
+__global__ __launch_bounds__(256) void gemm_join_kernel(const float *__restrict__ part, int splits, int64_t M, int64_t N, Epilogue ep) {
+    const int64_t per = (N + 3) / 4;
+    for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < M * per; i += (int64_t)gridDim.x * 256) {
+        const int64_t m = i / per, n = (i % per) * 4;
+        const int left = N - n < 4 ? (int)(N - n) : 4;
+        f32x4 z = {0.f, 0.f, 0.f, 0.f};
+        for (int s = 0; s < splits; ++s) z += load4(part, DETBOX_F32, ((int64_t)s * M + m) * N + n, left);
+        finish4(ep, m, n, N, z);
+    }
+}
+
+// dz = g * act'(pre) in the type of x with rows of ldz elements (zeros behind N), and partial column sums of the unrounded dz
+// per row slice.  A thread owns four columns of every slices-th group of rows.
 template <typename T>
 __global__ __launch_bounds__(256) void linear_slope_kernel(const void *g, int gdt, int64_t ldg, const T *__restrict__ pre, int act,
-                                                           int64_t M, int64_t N, int slices, T *__restrict__ dz,
-                                                           float *__restrict__ part) {
-    const int64_t c = (int64_t)blockIdx.x * 256 + threadIdx.x;
-    if (c >= N) return;
-    float a = 0.f;
-    for (int64_t row = blockIdx.y; row < M; row += slices) {
-        float v = load_as_float(g, gdt, row * ldg + c);
-        if (pre) v *= act_slope((float)pre[row * N + c], act);
-        if (dz) dz[row * N + c] = (T)v;
+                                                           int64_t M, int64_t N, int64_t ldz, int64_t rows_per_slice,
+                                                           T *__restrict__ dz, float *__restrict__ part) {
+    constexpr int DT = sizeof(T) == 4 ? DETBOX_F32 : std::is_same_v<T, __bf16> ? DETBOX_BF16 : DETBOX_F16;
+    const int64_t c = ((int64_t)blockIdx.x * 64 + (threadIdx.x & 63)) * 4;
+    const int left = N - c >= 4 ? 4 : N - c > 0 ? (int)(N - c) : 0;
+    f32x4 a = {0.f, 0.f, 0.f, 0.f};
+    const int64_t lo = blockIdx.y * rows_per_slice, hi = lo + rows_per_slice < M ? lo + rows_per_slice : M;
+    for (int64_t row = lo + (threadIdx.x >> 6); row < hi && c < ldz; row += 4) {
+        f32x4 v = load4(g, gdt, row * ldg + c, left);
+        if (pre) {
+            const f32x4 z = load4(pre, DT, row * N + c, left);
+#pragma unroll
+            for (int j = 0; j < 4; ++j) v[j] = j < left ? v[j] * act_slope(z[j], act) : 0.f;
+        }
+        if (dz) store4(dz, DT, row * ldz + c, ldz - c < 4 ? (int)(ldz - c) : 4, v);
         a += v;
     }
-    if (part) part[(int64_t)blockIdx.y * N + c] = a;
+    if (!part) return;
+    __shared__ f32x4 s[256];
+    s[threadIdx.x] = a;
+    __syncthreads();
+    if (threadIdx.x < 64 && left > 0) {
+        a = s[threadIdx.x] + s[threadIdx.x + 64] + s[threadIdx.x + 128] + s[threadIdx.x + 192];
+        store4(part, DETBOX_F32, (int64_t)blockIdx.y * N + c, left, a);
+    }
 }
 
 __global__ __launch_bounds__(256) void linear_bias_join_kernel(const float *__restrict__ part, int64_t N, int slices, int bdt,
                                                                void *gb) {
-    const int64_t c = (int64_t)blockIdx.x * 256 + threadIdx.x;
-    if (c >= N) return;
+    const int64_t c = (int64_t)blockIdx.x * 64 + (threadIdx.x & 63);
     float a = 0.f;
-    for (int sl = 0; sl < slices; ++sl) a += part[(int64_t)sl * N + c];
-    store_from_float(gb, bdt, c, a);
+    if (c < N)
+        for (int sl = threadIdx.x >> 6; sl < slices; sl += 4) a += part[(int64_t)sl * N + c];
+    __shared__ float s[256];
+    s[threadIdx.x] = a;
+    __syncthreads();
+    if (threadIdx.x < 64 && c < N) store_from_float(gb, bdt, c, s[threadIdx.x] + s[threadIdx.x + 64] + s[threadIdx.x + 128] + s[threadIdx.x + 192]);
 }
 
-int slices_of(int64_t rows) { return (int)(rows < 256 ? (rows < 1 ? 1 : rows) : 256); }
+// ---- host ----------------------------------------------------------------------------------------------------------------
 
 bool act_ok(int act) { return act >= DETBOX_ACTIVATION_NONE && act <= DETBOX_ACTIVATION_SIGMOID; }
 
+// How a product is cut.  Tiles of 256 x 256 while they alone fill the chip's 256 CUs; 128 x 128 otherwise, with the
+// contraction in pieces where there are fewer than two tiles per CU.
+struct Plan { bool big; int tiles_m, tiles_n, splits; int64_t steps_per_split; };
+Plan plan_of(int dtype, int64_t M, int64_t N, int64_t K) {
+    Plan p;
+    const int64_t step = 128 / (int64_t)dtype_size(dtype), steps = (K + step - 1) / step;
+    p.big = ((M + 255) / 256) * ((N + 255) / 256) >= 192;
+    const int64_t t = p.big ? 256 : 128;
+    p.tiles_m = (int)((M + t - 1) / t);
+    p.tiles_n = (int)((N + t - 1) / t);
+    int64_t splits = 1;
+    if (!p.big) {
+        splits = 512 / ((int64_t)p.tiles_m * p.tiles_n);
+        const int64_t most = steps / 4;                      // at least four steps each
+        splits = splits > most ? most : splits;
+        splits = splits < 1 ? 1 : splits > 512 ? 512 : splits;
+    }
+    p.steps_per_split = (steps + splits - 1) / splits;
+    p.splits = p.steps_per_split > 0 ? (int)((steps + p.steps_per_split - 1) / p.steps_per_split) : 1;
+    if (p.splits < 1) { p.splits = 1; p.steps_per_split = 1; }
+    return p;
+}
+size_t plan_bytes(const Plan &p, int64_t M, int64_t N) {
+    return p.splits > 1 ? align_up((size_t)p.splits * M * N * sizeof(float), 256) : 0;
+}
+
 template <typename T>
-void gemm(const T *A, int64_t am, int64_t ak, const T *B, int64_t bn, int64_t bk, int64_t M, int64_t N, int64_t K,
-          const Epilogue &ep, void *C, hipStream_t s) {
-    const int64_t tn = (N + TILE - 1) / TILE, tiles = (M + TILE - 1) / TILE * tn;
-    gemm_any_kernel<T><<<dim3((unsigned)(tiles < (1 << 20) ? tiles : (1 << 20))), dim3(256), 0, s>>>(A, am, ak, B, bn, bk, M, N, K, ep,
-                                                                                                     C, tn, tiles);
+bool whole_chunks(const void *p, int64_t ld, int64_t extent) {
+    return (uintptr_t)p % 16 == 0 && ld % VEC_OF<T> == 0 && extent % VEC_OF<T> == 0;
+}
+
+template <typename T, bool AX, bool BX, int BM, int BN, int WM, int WN, bool ALIGNED>
+int launch_gemm(const GemmArgs<T> &g, hipStream_t s) {
+    constexpr int WAVES = (BM / WM) * (BN / WN), HALF = WM < 64 ? WM : 64;
+    constexpr int BUFFERS = 2 * (BM + BN) * 128, OUT = WAVES * HALF * (WN + 4) * 4, LDS = BUFFERS > OUT ? BUFFERS : OUT;
+    auto kernel = gemm_kernel<T, AX, BX, BM, BN, WM, WN, ALIGNED>;
+    DETBOX_HIP(hipFuncSetAttribute(reinterpret_cast<const void *>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, LDS));
+    kernel<<<dim3((unsigned)(g.tiles_m * g.tiles_n), (unsigned)g.splits), dim3(WAVES * 64), LDS, s>>>(g);
+    DETBOX_LAUNCH_CHECK();
+    return DETBOX_OK;
+}
+
+template <typename T, bool AX, bool BX>
+int gemm(const Operand<T> &a, const Operand<T> &b, int64_t K, int dtype, const Epilogue &ep, void *workspace, hipStream_t s) {
+    const Plan p = plan_of(dtype, a.rows, b.rows, K);
+    const GemmArgs<T> g{a, b, K, p.tiles_m, p.tiles_n, p.splits, p.steps_per_split, ep, static_cast<float *>(workspace)};
+    const bool aligned = whole_chunks<T>(a.p, a.ld, a.extent) && whole_chunks<T>(b.p, b.ld, b.extent);
+    int rc;
+    if (p.big) rc = aligned ? launch_gemm<T, AX, BX, 256, 256, 128, 64, true>(g, s) : launch_gemm<T, AX, BX, 256, 256, 128, 64, false>(g, s);
+    else rc = aligned ? launch_gemm<T, AX, BX, 128, 128, 64, 64, true>(g, s) : launch_gemm<T, AX, BX, 128, 128, 64, 64, false>(g, s);
+    if (rc) return rc;
+    if (p.splits > 1) {
+        const int64_t jobs = (a.rows * ((b.rows + 3) / 4) + 255) / 256;
+        gemm_join_kernel<<<dim3((unsigned)(jobs < 65536 ? jobs : 65536)), dim3(256), 0, s>>>(g.part, p.splits, a.rows, b.rows, ep);
+        DETBOX_LAUNCH_CHECK();
+    }
+    return DETBOX_OK;
 }
 
 int check_linear(int dtype, int act, int64_t ldx, int64_t ldw, int64_t M, int64_t N, int64_t K) {
@@ -128,14 +478,33 @@ int check_linear(int dtype, int act, int64_t ldx, int64_t ldw, int64_t M, int64_
     DETBOX_CHECK_ARG(act_ok(act), "unknown activation");
     DETBOX_CHECK_ARG(M >= 0 && N >= 1 && K >= 1 && M < (1ll << 31) && N < (1ll << 31) && K < (1ll << 31), "bad size");
     DETBOX_CHECK_ARG(ldx >= K && ldw >= K, "row stride below the row length");
+    // tiles are counted in 32 bits in each of the three products
+    auto tiles = [](int64_t a, int64_t b) { return ((a + 127) / 128) * ((b + 127) / 128); };
+    DETBOX_CHECK_ARG(tiles(M, N) < (1ll << 23) && tiles(M, K) < (1ll << 23) && tiles(N, K) < (1ll << 23), "size too large");
     return DETBOX_OK;
+}
+
+int workspace_error(const char *who) {
+    set_error("%s: workspace missing, misaligned or too small", who);
+    return DETBOX_ERR_WORKSPACE;
+}
+
+// Row slices of the slope pass: about 2048 workgroups.
+struct Slices { int count; int64_t rows; };
+Slices slices_of(int64_t M, int64_t N) {
+    int64_t n = 2048 / ((N + 255) / 256);
+    const int64_t most = (M + 15) / 16;
+    n = n > most ? most : n;
+    n = n < 1 ? 1 : n;
+    const int64_t rows = M > 0 ? (M + n - 1) / n : 1;
+    return {(int)(M > 0 ? (M + rows - 1) / rows : 1), rows};
 }
 
 }  // namespace
 
 extern "C" size_t detbox_linear_workspace_bytes(int dtype, int64_t M, int64_t N, int64_t K) {
-    (void)dtype; (void)M; (void)N; (void)K;
-    return 0;
+    if (!dtype_ok(dtype) || M < 1 || N < 1 || K < 1) return 0;
+    return plan_bytes(plan_of(dtype, M, N, K), M, N);
 }
 
 extern "C" int detbox_linear_forward(int dtype, int activation, const void *x, int64_t ldx, const void *weight, int64_t ldw,
@@ -148,23 +517,28 @@ extern "C" int detbox_linear_forward(int dtype, int activation, const void *x, i
     DETBOX_CHECK_ARG(!residual || ldr >= N, "row stride below the row length");
     if (M == 0) return DETBOX_OK;
     DETBOX_CHECK_ARG(x && weight && y, "null pointer");
-    (void)workspace; (void)workspace_bytes;
+    const size_t need = detbox_linear_workspace_bytes(dtype, M, N, K);
+    if (need && (!workspace || (uintptr_t)workspace % 256 || workspace_bytes < need)) return workspace_error(__func__);
     hipStream_t s = static_cast<hipStream_t>(stream);
     ProfScope ps("linear_forward", s);
-    const Epilogue ep{bias, bias_dtype, residual, ldr, activation, pre_activation, out_dtype};
+    const Epilogue ep{bias, bias_dtype, residual, ldr, activation, pre_activation, dtype, y, out_dtype};
+    int rc = DETBOX_OK;
     with_dtype(dtype, [&](auto t) {
         using T = decltype(t);
-        gemm<T>(static_cast<const T *>(x), ldx, 1, static_cast<const T *>(weight), ldw, 1, M, N, K, ep, y, s);
+        rc = gemm<T, false, false>({static_cast<const T *>(x), ldx, M, K}, {static_cast<const T *>(weight), ldw, N, K}, K, dtype, ep,
+                                   workspace, s);
     });
-    DETBOX_LAUNCH_CHECK();
-    return DETBOX_OK;
+    return rc;
 }
 
 extern "C" size_t detbox_linear_backward_workspace_bytes(int dtype, int activation, int grad_dtype, int64_t M, int64_t N, int64_t K) {
     if (!dtype_ok(dtype) || M < 0 || N < 1 || K < 1) return 0;
-    size_t b = align_up((size_t)slices_of(M) * (size_t)N * sizeof(float), 256);
-    if (activation != DETBOX_ACTIVATION_NONE || grad_dtype != dtype) b += align_up((size_t)M * (size_t)N * dtype_size(dtype), 256);
-    return b;
+    (void)activation; (void)grad_dtype;
+    const int64_t vec = 16 / (int64_t)dtype_size(dtype), ldz = (N + vec - 1) / vec * vec;
+    size_t b = align_up((size_t)slices_of(M, N).count * (size_t)N * sizeof(float), 256);
+    b += align_up((size_t)M * (size_t)ldz * dtype_size(dtype), 256);
+    const size_t px = M ? plan_bytes(plan_of(dtype, M, K, N), M, K) : 0, pw = M ? plan_bytes(plan_of(dtype, N, K, M), N, K) : 0;
+    return b + (px > pw ? px : pw);
 }
 
 extern "C" int detbox_linear_backward(int dtype, int activation, int grad_dtype, const void *grad_y, int64_t ldg,
@@ -178,32 +552,38 @@ extern "C" int detbox_linear_backward(int dtype, int activation, int grad_dtype,
     DETBOX_CHECK_ARG(M == 0 || (grad_y && (activation == DETBOX_ACTIVATION_NONE || pre_activation)), "null pointer");
     DETBOX_CHECK_ARG(M == 0 || ((!grad_x || weight) && (!grad_weight || x)), "null pointer");
     if (!workspace || (uintptr_t)workspace % 256 ||
-        workspace_bytes < detbox_linear_backward_workspace_bytes(dtype, activation, grad_dtype, M, N, K)) {
-        set_error("%s: workspace missing, misaligned or too small", __func__);
-        return DETBOX_ERR_WORKSPACE;
-    }
+        workspace_bytes < detbox_linear_backward_workspace_bytes(dtype, activation, grad_dtype, M, N, K))
+        return workspace_error(__func__);
     hipStream_t s = static_cast<hipStream_t>(stream);
     ProfScope ps("linear_backward", s);
-    const int slices = slices_of(M);
+    const Slices sl = slices_of(M, N);
     Carver ws(workspace);
-    float *part = ws.take<float>((size_t)slices * N);
-    const bool slope = activation != DETBOX_ACTIVATION_NONE, convert = slope || grad_dtype != dtype;
-    const Epilogue plain{nullptr, 0, nullptr, 0, DETBOX_ACTIVATION_NONE, nullptr, dtype};
+    float *part = ws.take<float>((size_t)sl.count * N);
+    int rc = DETBOX_OK;
     with_dtype(dtype, [&](auto t) {
         using T = decltype(t);
-        T *dz = convert ? ws.take<T>((size_t)M * N) : nullptr;
-        if (convert || grad_bias)
-            linear_slope_kernel<T><<<dim3((unsigned)((N + 255) / 256), slices), dim3(256), 0, s>>>(
-                grad_y, grad_dtype, ldg, slope ? static_cast<const T *>(pre_activation) : nullptr, activation, M, N, slices, dz,
-                grad_bias ? part : nullptr);
+        const int64_t padded = (N + VEC_OF<T> - 1) / VEC_OF<T> * VEC_OF<T>;
+        T *dz = ws.take<T>((size_t)M * padded);
+        void *pieces = ws.take<char>(0);
+        const bool slope = activation != DETBOX_ACTIVATION_NONE;
+        // dz is written out where it is not g itself, or where g's rows start off 16 bytes
+        const bool convert = slope || grad_dtype != dtype || !whole_chunks<T>(grad_y, ldg, N);
+        if (M && (convert || grad_bias))
+            linear_slope_kernel<T><<<dim3((unsigned)((padded + 255) / 256), sl.count), dim3(256), 0, s>>>(
+                grad_y, grad_dtype, ldg, slope ? static_cast<const T *>(pre_activation) : nullptr, activation, M, N, padded, sl.rows,
+                convert ? dz : nullptr, grad_bias ? part : nullptr);
         const T *z = convert ? dz : static_cast<const T *>(grad_y);
-        const int64_t ldz = convert ? N : ldg;
-        if (grad_x && M) gemm<T>(z, ldz, 1, static_cast<const T *>(weight), 1, ldw, M, K, N, plain, grad_x, s);
-        if (grad_weight) gemm<T>(z, 1, ldz, static_cast<const T *>(x), 1, ldx, N, K, M, plain, grad_weight, s);
+        const int64_t ldz = convert ? padded : ldg, z_end = convert ? padded : N;
+        Epilogue ep{nullptr, 0, nullptr, 0, DETBOX_ACTIVATION_NONE, nullptr, 0, grad_x, dtype};
+        // the zeros behind N let the contraction over N run in whole chunks; the weight's rows end there
+        if (grad_x && M) rc = gemm<T, false, true>({z, ldz, M, z_end}, {static_cast<const T *>(weight), ldw, K, K}, N, dtype, ep, pieces, s);
+        ep.out = grad_weight;
+        if (grad_weight && !rc) rc = gemm<T, true, true>({z, ldz, N, z_end}, {static_cast<const T *>(x), ldx, K, K}, M, dtype, ep, pieces, s);
     });
+    if (rc) return rc;
     DETBOX_LAUNCH_CHECK();
     if (grad_bias) {
-        linear_bias_join_kernel<<<dim3((unsigned)((N + 255) / 256)), dim3(256), 0, s>>>(part, N, slices, bias_dtype, grad_bias);
+        linear_bias_join_kernel<<<dim3((unsigned)((N + 63) / 64)), dim3(256), 0, s>>>(part, N, M ? sl.count : 0, bias_dtype, grad_bias);
         DETBOX_LAUNCH_CHECK();
     }
     return DETBOX_OK;
