@@ -8,7 +8,7 @@
 // One tile kernel serves all three products.  Each operand lies in memory either along the contraction (x, W forward) or
 // across it (W in grad_x; dz and x in grad_W); both come into LDS as they lie, 16 bytes at a time, and only the read of a
 // fragment differs: a plain 16-byte read, or the transposing LDS read of 16-bit elements.
-#include "dtype.h"
+#include "columns.h"
 
 using namespace detbox;
 
@@ -398,18 +398,6 @@ __global__ __launch_bounds__(256) void linear_slope_kernel(const void *g, int gd
     }
 }
 
-__global__ __launch_bounds__(256) void linear_bias_join_kernel(const float *__restrict__ part, int64_t N, int slices, int bdt,
-                                                               void *gb) {
-    const int64_t c = (int64_t)blockIdx.x * 64 + (threadIdx.x & 63);
-    float a = 0.f;
-    if (c < N)
-        for (int sl = threadIdx.x >> 6; sl < slices; sl += 4) a += part[(int64_t)sl * N + c];
-    __shared__ float s[256];
-    s[threadIdx.x] = a;
-    __syncthreads();
-    if (threadIdx.x < 64 && c < N) store_from_float(gb, bdt, c, s[threadIdx.x] + s[threadIdx.x + 64] + s[threadIdx.x + 128] + s[threadIdx.x + 192]);
-}
-
 // ---- host ----------------------------------------------------------------------------------------------------------------
 
 bool act_ok(int act) { return act >= DETBOX_ACTIVATION_NONE && act <= DETBOX_ACTIVATION_SIGMOID; }
@@ -583,7 +571,7 @@ extern "C" int detbox_linear_backward(int dtype, int activation, int grad_dtype,
     if (rc) return rc;
     DETBOX_LAUNCH_CHECK();
     if (grad_bias) {
-        linear_bias_join_kernel<<<dim3((unsigned)((N + 63) / 64)), dim3(256), 0, s>>>(part, N, M ? sl.count : 0, bias_dtype, grad_bias);
+        column_join(part, M ? sl.count : 0, N, N, bias_dtype, grad_bias, nullptr, s);
         DETBOX_LAUNCH_CHECK();
     }
     return DETBOX_OK;
