@@ -148,6 +148,8 @@ __device__ inline int across_swizzle(int k) {
     return sizeof(T) == 2 ? (k & 3) | ((k >> 3) & 1) << 2 : (k >> 2) & 3;
 }
 
+__device__ const uint4 zero_chunk = {0, 0, 0, 0};
+
 // The chunks of one step that a thread brings in: idx = j * THREADS + tid is also the place in LDS.
 template <typename T, bool ACROSS, int ROWS, int THREADS, bool ALIGNED>
 struct Stager {
@@ -183,16 +185,17 @@ struct Stager {
             }
         }
     }
+    // Brings chunk j of the next step straight into LDS (aligned operands; chunks behind the contraction's end from a zero).
+    __device__ void dma(int j, int64_t k_left, char *lds) {
+        const void *p = src[j];
+        src[j] += step;
+        if (k_left < STEP_K<T> && at[j] >= k_left) p = &zero_chunk;
+        __builtin_amdgcn_global_load_lds((gptr_t)p, (lptr_t)(lds + (j * THREADS + (threadIdx.x & ~63)) * 16), 16, 0, 0);
+    }
     // Chunk j of the next step, which starts k_left elements before the contraction's end; zeros behind the end.
     __device__ detbox_u4 load(int j, int64_t k_left) {
         const T *p = src[j];
         src[j] = p + step;
-        if (ALIGNED) {
-            if (k_left >= STEP_K<T>) return *reinterpret_cast<const detbox_u4 *>(p);
-            detbox_u4 z = {0, 0, 0, 0};
-            if (at[j] < k_left) z = *reinterpret_cast<const detbox_u4 *>(p);
-            return z;
-        }
         int n = left[j];
         if (ACROSS) n = at[j] < k_left ? n : 0;
         else if (k_left - at[j] < VEC) n = k_left - at[j] < 0 ? 0 : (int)(k_left - at[j]);
@@ -267,6 +270,47 @@ __device__ inline void tile_of(int wg, int tiles_m, int tiles_n, int &tm, int &t
     tn = in / rows;
 }
 
+// The products of one step, from the buffer `cur` (A's rows first), while the next step comes into `nxt`.  The two pointers
+// are restrict: without it the compiler takes every LDS read for one that may want what is still on its way and waits for
+// the whole transfer first.  Reads and matrix instructions are interleaved by hand, the second half's reads under the first
+// half's products (8192^3 bf16: 997 us with staging through registers, 944 with the compiler's order, 892 so).
+template <typename T, bool AX, bool BX, int BM, int BN, int FM, int FN>
+__device__ __forceinline__ void multiply_step(const char *__restrict__ cur, int wm, int wn, f32x4 (&acc)[FM][FN]) {
+#pragma unroll
+    for (int ks = 0; ks < 2; ++ks) {
+        detbox_u4 fa[FM], fb[FN];
+#pragma unroll
+        for (int i = 0; i < FM; ++i) fa[i] = read_fragment<T, AX, BM>(cur, wm + i * 16, ks);
+#pragma unroll
+        for (int j = 0; j < FN; ++j) fb[j] = read_fragment<T, BX, BN>(cur + BM * 128, wn + j * 16, ks);
+#pragma unroll
+        for (int i = 0; i < FM; ++i)
+#pragma unroll
+            for (int j = 0; j < FN; ++j) acc[i][j] = multiply<T>(fb[j], fa[i], acc[i][j]);
+    }
+    if constexpr (sizeof(T) == 2) {
+        constexpr int READS = FM * (AX ? 2 : 1) + FN * (BX ? 2 : 1), EACH = FM * FN / READS;
+        __builtin_amdgcn_sched_group_barrier(0x100, READS, 0);
+#pragma unroll
+        for (int r = 0; r < READS; ++r) {
+            __builtin_amdgcn_sched_group_barrier(0x008, EACH, 0);
+            __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
+        }
+        __builtin_amdgcn_sched_group_barrier(0x008, 2 * FM * FN - READS * EACH, 0);
+    }
+}
+template <typename T, bool AX, bool BX, int BM, int BN, int FM, int FN, typename SA, typename SB>
+__device__ __forceinline__ void dma_step(const char *__restrict__ cur, char *__restrict__ nxt, SA &sa, SB &sb, bool more,
+                                         int64_t k_left, int wm, int wn, f32x4 (&acc)[FM][FN]) {
+    if (more) {
+#pragma unroll
+        for (int j = 0; j < SA::COUNT; ++j) sa.dma(j, k_left, nxt);
+#pragma unroll
+        for (int j = 0; j < SB::COUNT; ++j) sb.dma(j, k_left, nxt + BM * 128);
+    }
+    multiply_step<T, AX, BX, BM, BN, FM, FN>(cur, wm, wn, acc);
+}
+
 template <typename T, bool AX, bool BX, int BM, int BN, int WM, int WN, bool ALIGNED>
 __global__ __launch_bounds__((BM / WM) * (BN / WN) * 64) void gemm_kernel(GemmArgs<T> g) {
     constexpr int THREADS = (BM / WM) * (BN / WN) * 64, FM = WM / 16, FN = WN / 16;
@@ -286,54 +330,58 @@ __global__ __launch_bounds__((BM / WM) * (BN / WN) * 64) void gemm_kernel(GemmAr
     const int64_t k0 = s0 * STEP_K<T>;
     sa.init(g.a, m0, k0);
     sb.init(g.b, n0, k0);
-    detbox_u4 ra[sa.COUNT], rb[sb.COUNT];
-    auto fetch = [&](int64_t s) {
-        const int64_t k_left = g.K - k0 - s * STEP_K<T>;
-#pragma unroll
-        for (int j = 0; j < sa.COUNT; ++j) ra[j] = sa.load(j, k_left);
-#pragma unroll
-        for (int j = 0; j < sb.COUNT; ++j) rb[j] = sb.load(j, k_left);
-    };
-    auto put = [&](int buf) {
-        char *la = lds + buf * (A_BYTES + B_BYTES), *lb = la + A_BYTES;
-#pragma unroll
-        for (int j = 0; j < sa.COUNT; ++j) *reinterpret_cast<detbox_u4 *>(la + (j * THREADS + threadIdx.x) * 16) = ra[j];
-#pragma unroll
-        for (int j = 0; j < sb.COUNT; ++j) *reinterpret_cast<detbox_u4 *>(lb + (j * THREADS + threadIdx.x) * 16) = rb[j];
-    };
-
     f32x4 acc[FM][FN];
 #pragma unroll
     for (int i = 0; i < FM; ++i)
 #pragma unroll
         for (int j = 0; j < FN; ++j) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
 
-    if (steps > 0) {
-        fetch(0);
-        put(0);
-    }
-    __syncthreads();
-    for (int64_t s = 0; s < steps; ++s) {
-        if (s + 1 < steps) fetch(s + 1);
-        const char *la = lds + (s & 1) * (A_BYTES + B_BYTES), *lb = la + A_BYTES;
+    auto buffer = [&](int64_t i) { return lds + (i & 1) * (A_BYTES + B_BYTES); };
+    const int64_t k_all = g.K - k0;
+    if constexpr (ALIGNED) {
+        if (steps > 0) {
 #pragma unroll
-        for (int ks = 0; ks < 2; ++ks) {
-            detbox_u4 fa[FM], fb[FN];
+            for (int j = 0; j < sa.COUNT; ++j) sa.dma(j, k_all, lds);
 #pragma unroll
-            for (int i = 0; i < FM; ++i) fa[i] = read_fragment<T, AX, BM>(la, wm + i * 16, ks);
-#pragma unroll
-            for (int j = 0; j < FN; ++j) fb[j] = read_fragment<T, BX, BN>(lb, wn + j * 16, ks);
-#pragma unroll
-            for (int i = 0; i < FM; ++i)
-#pragma unroll
-                for (int j = 0; j < FN; ++j) acc[i][j] = multiply<T>(fb[j], fa[i], acc[i][j]);
+            for (int j = 0; j < sb.COUNT; ++j) sb.dma(j, k_all, lds + A_BYTES);
         }
-        if (s + 1 < steps) put((s + 1) & 1);
+        __builtin_amdgcn_s_waitcnt(0x0070);                  // vmcnt(0) lgkmcnt(0): what was on its way has arrived
         __syncthreads();
+        for (int64_t s = 0; s < steps; ++s) {
+            dma_step<T, AX, BX, BM, BN, FM, FN>(buffer(s), buffer(s + 1), sa, sb, s + 1 < steps, k_all - (s + 1) * STEP_K<T>, wm, wn, acc);
+            __builtin_amdgcn_s_waitcnt(0x0070);
+            __syncthreads();
+        }
+    } else {
+        // rows that start off 16 bytes or end inside a chunk: through registers
+        detbox_u4 ra[sa.COUNT], rb[sb.COUNT];
+        auto fetch = [&](int64_t s) {
+#pragma unroll
+            for (int j = 0; j < sa.COUNT; ++j) ra[j] = sa.load(j, k_all - s * STEP_K<T>);
+#pragma unroll
+            for (int j = 0; j < sb.COUNT; ++j) rb[j] = sb.load(j, k_all - s * STEP_K<T>);
+        };
+        auto put = [&](char *to) {
+#pragma unroll
+            for (int j = 0; j < sa.COUNT; ++j) *reinterpret_cast<detbox_u4 *>(to + (j * THREADS + threadIdx.x) * 16) = ra[j];
+#pragma unroll
+            for (int j = 0; j < sb.COUNT; ++j) *reinterpret_cast<detbox_u4 *>(to + A_BYTES + (j * THREADS + threadIdx.x) * 16) = rb[j];
+        };
+        if (steps > 0) {
+            fetch(0);
+            put(lds);
+        }
+        __syncthreads();
+        for (int64_t s = 0; s < steps; ++s) {
+            if (s + 1 < steps) fetch(s + 1);
+            multiply_step<T, AX, BX, BM, BN, FM, FN>(buffer(s), wm, wn, acc);
+            if (s + 1 < steps) put(buffer(s + 1));
+            __syncthreads();
+        }
     }
 
     // The sums go through LDS, 64 rows of the wave's part at a time, so that rows are written (and the residual read) in order.
-    constexpr int HALF = WM < 64 ? WM : 64, ROW = WN + PAD, LANES = WN / 4;
+    constexpr int HALF = WM < 64 ? WM : 64, ROW = WN + PAD, LANES = WN / 4, AT_ONCE = 64 / LANES;
     float *mine = reinterpret_cast<float *>(lds) + wave * (HALF * ROW);
     const int64_t M = g.a.rows, N = g.b.rows;
 #pragma unroll
@@ -345,7 +393,7 @@ __global__ __launch_bounds__((BM / WM) * (BN / WN) * 64) void gemm_kernel(GemmAr
             for (int j = 0; j < FN; ++j)
                 *reinterpret_cast<f32x4 *>(mine + (i * 16 + (lane & 15)) * ROW + j * 16 + (lane >> 4) * 4) = acc[h * (HALF / 16) + i][j];
         __builtin_amdgcn_wave_barrier();
-        for (int r = lane / LANES; r < HALF; r += 64 / LANES) {
+        for (int r = lane / LANES; r < HALF && lane < AT_ONCE * LANES; r += AT_ONCE) {
             const int64_t m = m0 + wm + h * HALF + r, n = n0 + wn + (lane % LANES) * 4;
             if (m >= M) break;
             const f32x4 z = *reinterpret_cast<const f32x4 *>(mine + r * ROW + (lane % LANES) * 4);
