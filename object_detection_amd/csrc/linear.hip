@@ -37,28 +37,23 @@ __device__ inline float normal_cdf(float z, float e) {
     return z < 0.f ? tail : 1.0f - tail;
 }
 
-__device__ inline float act_value(float z, int act) {
-    switch (act) {
-        case DETBOX_ACTIVATION_RELU: return z > 0.f ? z : (z != z ? z : 0.f);
-        case DETBOX_ACTIVATION_GELU: return z < -1e4f ? 0.f : z * normal_cdf(z, fast_exp(-0.5f * z * z));
-        case DETBOX_ACTIVATION_SILU: return z < -1e4f ? 0.f : z * sigmoid_f(z);
-        case DETBOX_ACTIVATION_SIGMOID: return sigmoid_f(z);
-    }
-    return z;
+__device__ inline float relu_f(float z) { return z > 0.f ? z : (z != z ? z : 0.f); }
+__device__ inline float gelu_f(float z) { return z < -1e4f ? 0.f : z * normal_cdf(z, fast_exp(-0.5f * z * z)); }
+__device__ inline float silu_f(float z) { return z < -1e4f ? 0.f : z * sigmoid_f(z); }
+// The derivatives; z is kept off the infinities, where the products would be 0 * inf.
+__device__ inline float bounded(float z) { return z > 1e4f ? 1e4f : (z < -1e4f ? -1e4f : z); }
+__device__ inline float relu_slope(float z) { return z > 0.f ? 1.f : (z != z ? z : 0.f); }
+__device__ inline float gelu_slope(float z) {
+    z = bounded(z);
+    const float e = fast_exp(-0.5f * z * z);
+    return fmaf(z * 0.39894228040143268f, e, normal_cdf(z, e));
 }
-
-// The derivative; z is kept off the infinities, where the products below would be 0 * inf.
-__device__ inline float act_slope(float z, int act) {
-    if (act == DETBOX_ACTIVATION_RELU) return z > 0.f ? 1.f : (z != z ? z : 0.f);
-    z = z > 1e4f ? 1e4f : (z < -1e4f ? -1e4f : z);
-    if (act == DETBOX_ACTIVATION_GELU) {
-        const float e = fast_exp(-0.5f * z * z);
-        return fmaf(z * 0.39894228040143268f, e, normal_cdf(z, e));
-    }
-    if (act == DETBOX_ACTIVATION_SILU) { const float p = sigmoid_f(z); return p * (1.0f + z * (1.0f - p)); }
-    if (act == DETBOX_ACTIVATION_SIGMOID) { const float p = sigmoid_f(z); return p * (1.0f - p); }
-    return 1.f;
+__device__ inline float silu_slope(float z) {
+    z = bounded(z);
+    const float p = sigmoid_f(z);
+    return p * (1.0f + z * (1.0f - p));
 }
+__device__ inline float sigmoid_slope(float z) { const float p = sigmoid_f(z); return p * (1.0f - p); }
 
 struct Epilogue {
     const void *bias; int bias_dtype;
@@ -68,6 +63,40 @@ struct Epilogue {
     void *out; int out_dtype;
 };
 
+// Four values with one (uniform) choice of the activation.
+#define DETBOX_FOUR(f) f32x4{f(z[0]), f(z[1]), f(z[2]), f(z[3])}
+__device__ inline f32x4 act4(f32x4 z, int act) {
+    switch (act) {
+        case DETBOX_ACTIVATION_RELU: return DETBOX_FOUR(relu_f);
+        case DETBOX_ACTIVATION_GELU: return DETBOX_FOUR(gelu_f);
+        case DETBOX_ACTIVATION_SILU: return DETBOX_FOUR(silu_f);
+        case DETBOX_ACTIVATION_SIGMOID: return DETBOX_FOUR(sigmoid_f);
+    }
+    return z;
+}
+__device__ inline f32x4 slope4(f32x4 z, int act) {
+    switch (act) {
+        case DETBOX_ACTIVATION_RELU: return DETBOX_FOUR(relu_slope);
+        case DETBOX_ACTIVATION_GELU: return DETBOX_FOUR(gelu_slope);
+        case DETBOX_ACTIVATION_SILU: return DETBOX_FOUR(silu_slope);
+        case DETBOX_ACTIVATION_SIGMOID: return DETBOX_FOUR(sigmoid_slope);
+    }
+    return f32x4{1.f, 1.f, 1.f, 1.f};
+}
+#undef DETBOX_FOUR
+
+// Four elements as they were loaded: a pack of fp32, or the first eight bytes of 16-bit ones.
+__device__ inline f32x4 widen4(detbox_u4 u, int dtype) {
+    if (dtype == DETBOX_F32) return __builtin_bit_cast(f32x4, u);
+    f32x4 v;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+        const uint16_t h = (uint16_t)(u[j >> 1] >> (16 * (j & 1)));
+        v[j] = dtype == DETBOX_BF16 ? __uint_as_float((uint32_t)h << 16) : (float)__builtin_bit_cast(_Float16, h);
+    }
+    return v;
+}
+
 // n <= 4 consecutive elements of a buffer whose type is known at run time, from any address of an element
 typedef uint32_t detbox_u2_at2 __attribute__((ext_vector_type(2), aligned(2), may_alias));
 __device__ inline f32x4 load4(const void *p, int dtype, int64_t i, int n) {
@@ -75,12 +104,7 @@ __device__ inline f32x4 load4(const void *p, int dtype, int64_t i, int n) {
     if (n >= 4) {
         if (dtype == DETBOX_F32) return __builtin_bit_cast(f32x4, load_raw<float>(static_cast<const float *>(p) + i));
         const detbox_u2_at2 u = *reinterpret_cast<const detbox_u2_at2 *>(static_cast<const uint16_t *>(p) + i);
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-            const uint16_t h = (uint16_t)(u[j >> 1] >> (16 * (j & 1)));
-            v[j] = dtype == DETBOX_BF16 ? __uint_as_float((uint32_t)h << 16) : (float)__builtin_bit_cast(_Float16, h);
-        }
-        return v;
+        return widen4(detbox_u4{u[0], u[1], 0, 0}, dtype);
     }
     for (int j = 0; j < n; ++j) v[j] = load_as_float(p, dtype, i + j);
     return v;
@@ -111,10 +135,7 @@ __device__ inline void finish4(const Epilogue &ep, int64_t m, int64_t n, int64_t
     if (left <= 0) return;
     if (ep.bias) z += load4(ep.bias, ep.bias_dtype, n, left);
     if (ep.pre) store4(ep.pre, ep.pre_dtype, m * N + n, left, z);
-    if (ep.act != DETBOX_ACTIVATION_NONE) {
-#pragma unroll
-        for (int j = 0; j < 4; ++j) z[j] = act_value(z[j], ep.act);
-    }
+    if (ep.act != DETBOX_ACTIVATION_NONE) z = act4(z, ep.act);
     if (ep.residual) z += load4(ep.residual, ep.out_dtype, m * ep.ldr + n, left);
     store4(ep.out, ep.out_dtype, m * N + n, left, z);
 }
@@ -383,7 +404,9 @@ __global__ __launch_bounds__((BM / WM) * (BN / WN) * 64) void gemm_kernel(GemmAr
     // The sums go through LDS, 64 rows of the wave's part at a time, so that rows are written (and the residual read) in order.
     constexpr int HALF = WM < 64 ? WM : 64, ROW = WN + PAD, LANES = WN / 4, AT_ONCE = 64 / LANES;
     float *mine = reinterpret_cast<float *>(lds) + wave * (HALF * ROW);
-    const int64_t M = g.a.rows, N = g.b.rows;
+    const int64_t M = g.a.rows, N = g.b.rows, n = n0 + wn + (lane % LANES) * 4;
+    const int left = lane >= AT_ONCE * LANES ? 0 : N - n >= 4 ? 4 : N > n ? (int)(N - n) : 0;
+    const f32x4 bias = g.ep.bias ? load4(g.ep.bias, g.ep.bias_dtype, n, left) : f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
     for (int h = 0; h < WM / HALF; ++h) {
         if (h) __builtin_amdgcn_wave_barrier();
@@ -393,12 +416,43 @@ __global__ __launch_bounds__((BM / WM) * (BN / WN) * 64) void gemm_kernel(GemmAr
             for (int j = 0; j < FN; ++j)
                 *reinterpret_cast<f32x4 *>(mine + (i * 16 + (lane & 15)) * ROW + j * 16 + (lane >> 4) * 4) = acc[h * (HALF / 16) + i][j];
         __builtin_amdgcn_wave_barrier();
-        for (int r = lane / LANES; r < HALF && lane < AT_ONCE * LANES; r += AT_ONCE) {
-            const int64_t m = m0 + wm + h * HALF + r, n = n0 + wn + (lane % LANES) * 4;
-            if (m >= M) break;
-            const f32x4 z = *reinterpret_cast<const f32x4 *>(mine + r * ROW + (lane % LANES) * 4);
-            if (g.splits == 1) finish4(g.ep, m, n, N, z);
-            else if (n < N) store4(g.part, DETBOX_F32, ((int64_t)split * M + m) * N + n, N - n < 4 ? (int)(N - n) : 4, z);
+        // a batch of rows at a time: the residual's loads of a batch are on their way together
+        constexpr int TURNS = (HALF + AT_ONCE - 1) / AT_ONCE, U = TURNS < 8 ? TURNS : 8;
+        for (int t = 0; t < TURNS; t += U) {
+            detbox_u4 raw[U];
+            auto row_of = [&](int u) { return (t + u) * AT_ONCE + lane / LANES; };
+            auto alive = [&](int u) { return row_of(u) < HALF && m0 + wm + h * HALF + row_of(u) < M; };
+            if (g.ep.residual && left == 4) {
+                const int64_t at = (m0 + wm + h * HALF + row_of(0)) * g.ep.ldr + n, by = (int64_t)AT_ONCE * g.ep.ldr;
+                if (g.ep.out_dtype == DETBOX_F32) {
+#pragma unroll
+                    for (int u = 0; u < U; ++u)
+                        if (alive(u)) raw[u] = load_raw<float>(static_cast<const float *>(g.ep.residual) + at + u * by);
+                } else {
+#pragma unroll
+                    for (int u = 0; u < U; ++u)
+                        if (alive(u)) {
+                            const detbox_u2_at2 w = *reinterpret_cast<const detbox_u2_at2 *>(static_cast<const uint16_t *>(g.ep.residual) + at + u * by);
+                            raw[u][0] = w[0];
+                            raw[u][1] = w[1];
+                        }
+                }
+            }
+#pragma unroll
+            for (int u = 0; u < U; ++u) {
+                if (left <= 0 || !alive(u)) continue;
+                const int64_t m = m0 + wm + h * HALF + row_of(u);
+                f32x4 z = *reinterpret_cast<const f32x4 *>(mine + row_of(u) * ROW + (lane % LANES) * 4);
+                if (g.splits > 1) {
+                    store4(g.part, DETBOX_F32, ((int64_t)split * M + m) * N + n, left, z);
+                    continue;
+                }
+                z += bias;
+                if (g.ep.pre) store4(g.ep.pre, g.ep.pre_dtype, m * N + n, left, z);
+                if (g.ep.act != DETBOX_ACTIVATION_NONE) z = act4(z, g.ep.act);
+                if (g.ep.residual) z += left == 4 ? widen4(raw[u], g.ep.out_dtype) : load4(g.ep.residual, g.ep.out_dtype, m * g.ep.ldr + n, left);
+                store4(g.ep.out, g.ep.out_dtype, m * N + n, left, z);
+            }
         }
     }
 }
@@ -429,9 +483,7 @@ __global__ __launch_bounds__(256) void linear_slope_kernel(const void *g, int gd
     for (int64_t row = lo + (threadIdx.x >> 6); row < hi && c < ldz; row += 4) {
         f32x4 v = load4(g, gdt, row * ldg + c, left);
         if (pre) {
-            const f32x4 z = load4(pre, DT, row * N + c, left);
-#pragma unroll
-            for (int j = 0; j < 4; ++j) v[j] = j < left ? v[j] * act_slope(z[j], act) : 0.f;
+            v *= slope4(load4(pre, DT, row * N + c, left), act);          // v is 0 behind N
         }
         if (dz) store4(dz, DT, row * ldz + c, ldz - c < 4 ? (int)(ldz - c) : 4, v);
         a += v;
