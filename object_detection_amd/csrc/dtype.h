@@ -98,6 +98,15 @@ __device__ inline void load_packs_to_end(float (&v)[U][VEC_OF<T>], const T *row,
             }
         }
 }
+// A pack whose first `by` elements are not wanted (0 < by): the rest moved down, zeros behind them.
+template <typename T>
+__device__ inline detbox_u4 moved_down(detbox_u4 u, int64_t by) {
+    if (by >= VEC_OF<T>) return detbox_u4{0, 0, 0, 0};
+    const int bits = (int)by * 8 * (int)sizeof(T);
+    const unsigned long long lo = ((unsigned long long)u[1] << 32) | u[0], hi = ((unsigned long long)u[3] << 32) | u[2];
+    const unsigned long long l = bits >= 64 ? hi >> (bits - 64) : (lo >> bits) | (hi << (64 - bits)), h = bits >= 64 ? 0 : hi >> bits;
+    return detbox_u4{(uint32_t)l, (uint32_t)(l >> 32), (uint32_t)h, (uint32_t)(h >> 32)};
+}
 // The first n of a pack; the rest reads as `fill` and is not touched in memory.
 template <typename T>
 __device__ inline void load_pack(float (&v)[VEC_OF<T>], const T *p, int64_t n, float fill) {

@@ -457,44 +457,163 @@ __global__ __launch_bounds__((BM / WM) * (BN / WN) * 64) void gemm_kernel(GemmAr
     }
 }
 
-// Adds the pieces of the contraction in order and applies the epilogue.
+// Adds the pieces of the contraction in a fixed order and applies the epilogue.  SLICES threads share an output: 16 where there
+// are many pieces of a small product (256 pieces of 81 x 256: 82 us with one thread per output, 9 us so).
+template <int SLICES>
 __global__ __launch_bounds__(256) void gemm_join_kernel(const float *__restrict__ part, int splits, int64_t M, int64_t N, Epilogue ep) {
-    const int64_t per = (N + 3) / 4;
-    for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < M * per; i += (int64_t)gridDim.x * 256) {
-        const int64_t m = i / per, n = (i % per) * 4;
-        const int left = N - n < 4 ? (int)(N - n) : 4;
+    constexpr int OUT = 256 / SLICES;
+    __shared__ f32x4 sums[SLICES > 1 ? 256 : 1];
+    const int64_t per = (N + 3) / 4, total = M * per;
+    const int slice = threadIdx.x / OUT;
+    for (int64_t i0 = (int64_t)blockIdx.x * OUT; i0 < total; i0 += (int64_t)gridDim.x * OUT) {
+        const int64_t i = i0 + threadIdx.x % OUT, m = i / per, n = (i % per) * 4;
+        const int left = i >= total ? 0 : N - n < 4 ? (int)(N - n) : 4;
         f32x4 z = {0.f, 0.f, 0.f, 0.f};
-        for (int s = 0; s < splits; ++s) z += load4(part, DETBOX_F32, ((int64_t)s * M + m) * N + n, left);
-        finish4(ep, m, n, N, z);
+        if (left > 0) {
+#pragma unroll 4
+            for (int s = slice; s < splits; s += SLICES) z += load4(part, DETBOX_F32, ((int64_t)s * M + m) * N + n, left);
+        }
+        if constexpr (SLICES > 1) {
+            sums[threadIdx.x] = z;
+            __syncthreads();
+            if (slice == 0) {
+#pragma unroll
+                for (int s = 1; s < SLICES; ++s) z += sums[s * OUT + threadIdx.x];
+            }
+            __syncthreads();
+        }
+        if (slice == 0 && left > 0) finish4(ep, m, n, N, z);
     }
 }
 
 // dz = g * act'(pre) in the type of x with rows of ldz elements (zeros behind N), and partial column sums of the unrounded dz
-// per row slice.  A thread owns four columns of every slices-th group of rows.
-template <typename T>
+// per row slice.  LANES lanes share a row, four columns each; HBM bound.
+template <typename T, int LANES>
 __global__ __launch_bounds__(256) void linear_slope_kernel(const void *g, int gdt, int64_t ldg, const T *__restrict__ pre, int act,
                                                            int64_t M, int64_t N, int64_t ldz, int64_t rows_per_slice,
                                                            T *__restrict__ dz, float *__restrict__ part) {
-    constexpr int DT = sizeof(T) == 4 ? DETBOX_F32 : std::is_same_v<T, __bf16> ? DETBOX_BF16 : DETBOX_F16;
-    const int64_t c = ((int64_t)blockIdx.x * 64 + (threadIdx.x & 63)) * 4;
-    const int left = N - c >= 4 ? 4 : N - c > 0 ? (int)(N - c) : 0;
+    constexpr int DT = sizeof(T) == 4 ? DETBOX_F32 : std::is_same_v<T, __bf16> ? DETBOX_BF16 : DETBOX_F16, ROWS = 256 / LANES;
+    const int lane = threadIdx.x % LANES;
+    const int64_t c = ((int64_t)blockIdx.x * LANES + lane) * 4;
+    const int left = N - c >= 4 ? 4 : N - c > 0 ? (int)(N - c) : 0, room = ldz - c < 4 ? (int)(ldz - c) : 4;
     f32x4 a = {0.f, 0.f, 0.f, 0.f};
     const int64_t lo = blockIdx.y * rows_per_slice, hi = lo + rows_per_slice < M ? lo + rows_per_slice : M;
-    for (int64_t row = lo + (threadIdx.x >> 6); row < hi && c < ldz; row += 4) {
-        f32x4 v = load4(g, gdt, row * ldg + c, left);
-        if (pre) {
-            v *= slope4(load4(pre, DT, row * N + c, left), act);          // v is 0 behind N
+    if (c < ldz) {
+#pragma unroll 2
+        for (int64_t row = lo + threadIdx.x / LANES; row < hi; row += ROWS) {
+            f32x4 v = load4(g, gdt, row * ldg + c, left);
+            if (pre) v *= slope4(load4(pre, DT, row * N + c, left), act);          // v is 0 behind N
+            if (dz) store4(dz, DT, row * ldz + c, room, v);
+            a += v;
         }
-        if (dz) store4(dz, DT, row * ldz + c, ldz - c < 4 ? (int)(ldz - c) : 4, v);
-        a += v;
     }
     if (!part) return;
     __shared__ f32x4 s[256];
     s[threadIdx.x] = a;
     __syncthreads();
-    if (threadIdx.x < 64 && left > 0) {
-        a = s[threadIdx.x] + s[threadIdx.x + 64] + s[threadIdx.x + 128] + s[threadIdx.x + 192];
+    if (threadIdx.x < LANES && left > 0) {
+        for (int r = 1; r < ROWS; ++r) a += s[r * LANES + threadIdx.x];
         store4(part, DETBOX_F32, (int64_t)blockIdx.y * N + c, left, a);
+    }
+}
+
+// ---- many rows against few columns -----------------------------------------------------------------------------------------
+
+// B (all columns, the whole contraction) stays in LDS for the workgroup's life, in the order in which fragments are read; the
+// waves stream rows of A straight into registers, 16 MF at a time, each on its own: no barrier after the set-up, and what
+// bounds it is the read of A and the write of C.  RetinaNet's class logits (480348 x 256 bf16 by 81, fp32 out): 202 us with
+// tiles of 256 x 256 that drain their pipeline every four steps, 89 us = 4.5 TB/s so.
+constexpr int RES_BLOCK = 512, RES_LDS = 128 * 1024;
+
+template <typename T, bool BX, int MF, int NF>
+__global__ __launch_bounds__(RES_BLOCK, NF > 6 ? 2 : 4) void gemm_resident_kernel(const Operand<T> a, const Operand<T> b, int64_t K,
+                                                                                 int groups, Epilogue ep) {
+    constexpr int VEC = VEC_OF<T>, KF = 4 * VEC, CHUNK = 8 / MF > 4 ? 8 : 4;       // contraction of one fragment; fragments in flight
+    extern __shared__ __attribute__((aligned(16))) char lds[];
+    const int lane = threadIdx.x & 63, r = lane & 15, q = lane >> 4;
+    const int64_t M = a.rows, N = b.rows;
+    const int kf = (int)((K + KF - 1) / KF), all = groups * NF;
+    for (int i = threadIdx.x; i < kf * all * 64; i += RES_BLOCK) {
+        const int f = i >> 6, l = i & 63;
+        const int64_t n = (f % all) * 16 + (l & 15), k = (int64_t)(f / all) * KF + (l >> 4) * VEC;
+        detbox_u4 u = {0, 0, 0, 0};
+        if (BX) {
+            T e[VEC];
+#pragma unroll
+            for (int j = 0; j < VEC; ++j) e[j] = b.p[(k + j < K ? k + j : K - 1) * b.ld + (n < N ? n : N - 1)];
+#pragma unroll
+            for (int j = 0; j < VEC; ++j)
+                if (n >= N || k + j >= K) e[j] = (T)0.f;
+            __builtin_memcpy(&u, e, 16);
+        } else if (n < N && k < K) {
+            u = load_raw<T>(b.p + n * b.ld + (k + VEC <= K ? k : K - VEC));
+            if (k + VEC > K) u = moved_down<T>(u, k + VEC - K);
+        }
+        *reinterpret_cast<detbox_u4 *>(lds + i * 16) = u;
+    }
+    __syncthreads();
+    const int64_t blocks = (M + 16 * MF - 1) / (16 * MF), waves = (int64_t)gridDim.x * (RES_BLOCK / 64);
+    for (int64_t rb = (int64_t)blockIdx.x * (RES_BLOCK / 64) + (threadIdx.x >> 6); rb < blocks; rb += waves) {
+        const T *row[MF];
+#pragma unroll
+        for (int i = 0; i < MF; ++i) {
+            int64_t m = rb * 16 * MF + i * 16 + r;
+            m = m < M ? m : M - 1;                              // rows that do not exist: any values
+            row[i] = a.p + m * a.ld;
+        }
+        detbox_u4 fa[CHUNK][MF];
+        for (int g = 0; g < groups; ++g) {
+            // Opaque copies: what depends on the lane only would otherwise be computed once for every fragment and kept, some
+            // hundred registers of it.
+            int own = lane, quarter = q;
+            asm volatile("" : "+v"(own), "+v"(quarter));
+            f32x4 acc[MF][NF];
+#pragma unroll
+            for (int i = 0; i < MF; ++i)
+#pragma unroll
+                for (int j = 0; j < NF; ++j) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
+            for (int c0 = 0; c0 < kf; c0 += CHUNK) {
+                if (g == 0 || kf > CHUNK) {                              // a short contraction's rows are kept for all groups
+#pragma unroll
+                    for (int c = 0; c < CHUNK; ++c)
+#pragma unroll
+                        for (int i = 0; i < MF; ++i) {
+                            const int64_t k = (int64_t)(c0 + c) * KF + quarter * VEC;
+                            // the last whole pack where the row ends earlier; K >= VEC here
+                            fa[c][i] = load_raw_nt<T>(row[i] + (k + VEC <= K ? k : K - VEC));
+                        }
+                    if ((int64_t)(c0 + CHUNK) * KF > K) {
+#pragma unroll
+                        for (int c = 0; c < CHUNK; ++c) {
+                            const int64_t k = (int64_t)(c0 + c) * KF + quarter * VEC;
+                            if (k + VEC > K) {
+#pragma unroll
+                                for (int i = 0; i < MF; ++i) fa[c][i] = moved_down<T>(fa[c][i], k + VEC - K);
+                            }
+                        }
+                    }
+                }
+#pragma unroll
+                for (int c = 0; c < CHUNK; ++c) {
+                    if (c0 + c >= kf) break;
+                    const char *at = lds + (((c0 + c) * all + g * NF) * 64 + own) * 16;
+#pragma unroll
+                    for (int j = 0; j < NF; ++j) {
+                        const detbox_u4 fb = *reinterpret_cast<const detbox_u4 *>(at + j * 1024);
+#pragma unroll
+                        for (int i = 0; i < MF; ++i) acc[i][j] = multiply<T>(fb, fa[c][i], acc[i][j]);
+                    }
+                }
+            }
+#pragma unroll
+            for (int i = 0; i < MF; ++i) {
+                const int64_t m = rb * 16 * MF + i * 16 + r;
+                if (m < M) {
+#pragma unroll
+                    for (int j = 0; j < NF; ++j) finish4(ep, m, (g * NF + j) * 16 + quarter * 4, N, acc[i][j]);
+                }
+            }
+        }
     }
 }
 
@@ -544,8 +663,42 @@ int launch_gemm(const GemmArgs<T> &g, hipStream_t s) {
     return DETBOX_OK;
 }
 
+// Whether B fits LDS whole (128 KB) and there are rows enough to pay for bringing it there.  Measured in bf16 against the tiles
+// (us): 32768 x 512 by 128 22 / 33, 16384 x 256 by 81 13 / 13, 8192 x 1024 by 32 22 / 12; with more columns it only pays
+// where a short contraction leaves the tiles' pipeline no steps: 120087 x 64 by 512 55 / 64, 32768 x 64 by 512 30 / 19,
+// 120087 x 256 by 256 74 / 45.
+int resident_columns(int64_t N) { return (int)(N <= 32 ? 2 : N <= 64 ? 4 : N <= 96 ? 6 : (N + 127) / 128 * 8); }
+bool resident(int dtype, int64_t M, int64_t N, int64_t K) {
+    const int64_t vec = 16 / (int64_t)dtype_size(dtype), kf = (K + 4 * vec - 1) / (4 * vec);
+    if (K < vec || N > 512 || kf * resident_columns(N) * 1024 > RES_LDS) return false;
+    return N <= 128 ? M >= 32768 : M >= 98304 && K * (int64_t)dtype_size(dtype) <= 256;
+}
+
+template <typename T, bool BX, int MF, int NF>
+int launch_resident(const Operand<T> &a, const Operand<T> &b, int64_t K, const Epilogue &ep, hipStream_t s) {
+    constexpr int64_t KF = 4 * VEC_OF<T>;
+    const int all = resident_columns(b.rows), lds = (int)((K + KF - 1) / KF * all * 1024);
+    auto kernel = gemm_resident_kernel<T, BX, MF, NF>;
+    DETBOX_HIP(hipFuncSetAttribute(reinterpret_cast<const void *>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, RES_LDS));
+    const int64_t blocks = (a.rows + 16 * MF - 1) / (16 * MF), wgs = (blocks + RES_BLOCK / 64 - 1) / (RES_BLOCK / 64);
+    const int64_t most = lds > 80 * 1024 || NF > 6 ? 256 : 512;         // one or two per CU
+    kernel<<<dim3((unsigned)(wgs < most ? wgs : most)), dim3(RES_BLOCK), lds, s>>>(a, b, K, all / NF, ep);
+    DETBOX_LAUNCH_CHECK();
+    return DETBOX_OK;
+}
+template <typename T, bool BX>
+int gemm_resident(const Operand<T> &a, const Operand<T> &b, int64_t K, const Epilogue &ep, hipStream_t s) {
+    if (b.rows <= 32) return launch_resident<T, BX, 2, 2>(a, b, K, ep, s);
+    if (b.rows <= 64) return launch_resident<T, BX, 2, 4>(a, b, K, ep, s);
+    if (b.rows <= 96) return launch_resident<T, BX, 2, 6>(a, b, K, ep, s);
+    return launch_resident<T, BX, 2, 8>(a, b, K, ep, s);
+}
+
 template <typename T, bool AX, bool BX>
 int gemm(const Operand<T> &a, const Operand<T> &b, int64_t K, int dtype, const Epilogue &ep, void *workspace, hipStream_t s) {
+    if constexpr (!AX) {
+        if (resident(dtype, a.rows, b.rows, K)) return gemm_resident<T, BX>(a, b, K, ep, s);
+    }
     const Plan p = plan_of(dtype, a.rows, b.rows, K);
     const GemmArgs<T> g{a, b, K, p.tiles_m, p.tiles_n, p.splits, p.steps_per_split, ep, static_cast<float *>(workspace)};
     const bool aligned = whole_chunks<T>(a.p, a.ld, a.extent) && whole_chunks<T>(b.p, b.ld, b.extent);
@@ -554,8 +707,9 @@ int gemm(const Operand<T> &a, const Operand<T> &b, int64_t K, int dtype, const E
     else rc = aligned ? launch_gemm<T, AX, BX, 128, 128, 64, 64, true>(g, s) : launch_gemm<T, AX, BX, 128, 128, 64, 64, false>(g, s);
     if (rc) return rc;
     if (p.splits > 1) {
-        const int64_t jobs = (a.rows * ((b.rows + 3) / 4) + 255) / 256;
-        gemm_join_kernel<<<dim3((unsigned)(jobs < 65536 ? jobs : 65536)), dim3(256), 0, s>>>(g.part, p.splits, a.rows, b.rows, ep);
+        const int64_t outs = a.rows * ((b.rows + 3) / 4);
+        if (p.splits >= 16) gemm_join_kernel<16><<<dim3((unsigned)(outs < 16 << 16 ? (outs + 15) / 16 : 65536)), dim3(256), 0, s>>>(g.part, p.splits, a.rows, b.rows, ep);
+        else gemm_join_kernel<1><<<dim3((unsigned)(outs < 256 << 16 ? (outs + 255) / 256 : 65536)), dim3(256), 0, s>>>(g.part, p.splits, a.rows, b.rows, ep);
         DETBOX_LAUNCH_CHECK();
     }
     return DETBOX_OK;
@@ -656,10 +810,17 @@ extern "C" int detbox_linear_backward(int dtype, int activation, int grad_dtype,
         const bool slope = activation != DETBOX_ACTIVATION_NONE;
         // dz is written out where it is not g itself, or where g's rows start off 16 bytes
         const bool convert = slope || grad_dtype != dtype || !whole_chunks<T>(grad_y, ldg, N);
-        if (M && (convert || grad_bias))
-            linear_slope_kernel<T><<<dim3((unsigned)((padded + 255) / 256), sl.count), dim3(256), 0, s>>>(
-                grad_y, grad_dtype, ldg, slope ? static_cast<const T *>(pre_activation) : nullptr, activation, M, N, padded, sl.rows,
-                convert ? dz : nullptr, grad_bias ? part : nullptr);
+        if (M && (convert || grad_bias)) {
+            auto launch = [&](auto lanes) {
+                constexpr int LANES = decltype(lanes)::value;
+                linear_slope_kernel<T, LANES><<<dim3((unsigned)((padded + LANES * 4 - 1) / (LANES * 4)), sl.count), dim3(256), 0, s>>>(
+                    grad_y, grad_dtype, ldg, slope ? static_cast<const T *>(pre_activation) : nullptr, activation, M, N, padded, sl.rows,
+                    convert ? dz : nullptr, grad_bias ? part : nullptr);
+            };
+            if (padded <= 32) launch(std::integral_constant<int, 8>{});
+            else if (padded <= 128) launch(std::integral_constant<int, 32>{});
+            else launch(std::integral_constant<int, 64>{});
+        }
         const T *z = convert ? dz : static_cast<const T *>(grad_y);
         const int64_t ldz = convert ? padded : ldg, z_end = convert ? padded : N;
         Epilogue ep{nullptr, 0, nullptr, 0, DETBOX_ACTIVATION_NONE, nullptr, 0, grad_x, dtype};
