@@ -294,7 +294,8 @@ __device__ inline void tile_of(int wg, int tiles_m, int tiles_n, int &tm, int &t
 // The products of one step, from the buffer `cur` (A's rows first), while the next step comes into `nxt`.  The two pointers
 // are restrict: without it the compiler takes every LDS read for one that may want what is still on its way and waits for
 // the whole transfer first.  Reads and matrix instructions are interleaved by hand, the second half's reads under the first
-// half's products (8192^3 bf16: 997 us with staging through registers, 944 with the compiler's order, 892 so).
+// half's products.  8192^3 bf16 forward: 997 us with staging through registers, 944 with the compiler's order, 860 so =
+// 1.28 PFLOP/s (grad_x 1.30, grad_W 1.31).
 template <typename T, bool AX, bool BX, int BM, int BN, int FM, int FN>
 __device__ __forceinline__ void multiply_step(const char *__restrict__ cur, int wm, int wn, f32x4 (&acc)[FM][FN]) {
 #pragma unroll
@@ -360,19 +361,21 @@ __global__ __launch_bounds__((BM / WM) * (BN / WN) * 64) void gemm_kernel(GemmAr
     auto buffer = [&](int64_t i) { return lds + (i & 1) * (A_BYTES + B_BYTES); };
     const int64_t k_all = g.K - k0;
     if constexpr (ALIGNED) {
-        if (steps > 0) {
+        auto issue = [&](int64_t s) {
 #pragma unroll
-            for (int j = 0; j < sa.COUNT; ++j) sa.dma(j, k_all, lds);
+            for (int j = 0; j < sa.COUNT; ++j) sa.dma(j, k_all - s * STEP_K<T>, buffer(s));
 #pragma unroll
-            for (int j = 0; j < sb.COUNT; ++j) sb.dma(j, k_all, lds + A_BYTES);
-        }
-        __builtin_amdgcn_s_waitcnt(0x0070);                  // vmcnt(0) lgkmcnt(0): what was on its way has arrived
-        __syncthreads();
+            for (int j = 0; j < sb.COUNT; ++j) sb.dma(j, k_all - s * STEP_K<T>, buffer(s) + A_BYTES);
+        };
+        if (steps > 0) issue(0);
         for (int64_t s = 0; s < steps; ++s) {
+            __builtin_amdgcn_s_waitcnt(0x0070);              // vmcnt(0) lgkmcnt(0): step s has arrived, what was read is here
+            asm volatile("" ::: "memory");
+            __builtin_amdgcn_s_barrier();                    // ... in every wave: the other buffer is free
+            asm volatile("" ::: "memory");
             dma_step<T, AX, BX, BM, BN, FM, FN>(buffer(s), buffer(s + 1), sa, sb, s + 1 < steps, k_all - (s + 1) * STEP_K<T>, wm, wn, acc);
-            __builtin_amdgcn_s_waitcnt(0x0070);
-            __syncthreads();
         }
+        __syncthreads();
     } else {
         // rows that start off 16 bytes or end inside a chunk: through registers
         detbox_u4 ra[sa.COUNT], rb[sb.COUNT];
@@ -621,13 +624,16 @@ __global__ __launch_bounds__(RES_BLOCK, NF > 6 ? 2 : 4) void gemm_resident_kerne
 
 bool act_ok(int act) { return act >= DETBOX_ACTIVATION_NONE && act <= DETBOX_ACTIVATION_SIGMOID; }
 
-// How a product is cut.  Tiles of 256 x 256 while they alone fill the chip's 256 CUs; 128 x 128 otherwise, with the
-// contraction in pieces where there are fewer than two tiles per CU.
+// How a product is cut.  Tiles of 256 x 256 (eight waves of 128 x 64, one workgroup per CU) where they alone fill the chip and
+// have steps enough to hide their start and end; tiles of 128 x 128 (eight waves of 64 x 32, two workgroups per CU)
+// otherwise, with the contraction in pieces where there are fewer than two tiles per CU.  Measured (bf16, us, large / small):
+// 8192^3 860 / 1043, 4096^3 115 / 132, 8192 x 1024 by 8192 149 / 153, 8192 x 512 by 8192 103 / 95, 65536 x 256 by 256
+// 24 / 21, 2048^3 (64 large tiles) 59 / 31.
 struct Plan { bool big; int tiles_m, tiles_n, splits; int64_t steps_per_split; };
 Plan plan_of(int dtype, int64_t M, int64_t N, int64_t K) {
     Plan p;
     const int64_t step = 128 / (int64_t)dtype_size(dtype), steps = (K + step - 1) / step;
-    p.big = ((M + 255) / 256) * ((N + 255) / 256) >= 192;
+    p.big = ((M + 255) / 256) * ((N + 255) / 256) >= 192 && steps > 8;
     const int64_t t = p.big ? 256 : 128;
     p.tiles_m = (int)((M + t - 1) / t);
     p.tiles_n = (int)((N + t - 1) / t);
@@ -704,7 +710,7 @@ int gemm(const Operand<T> &a, const Operand<T> &b, int64_t K, int dtype, const E
     const bool aligned = whole_chunks<T>(a.p, a.ld, a.extent) && whole_chunks<T>(b.p, b.ld, b.extent);
     int rc;
     if (p.big) rc = aligned ? launch_gemm<T, AX, BX, 256, 256, 128, 64, true>(g, s) : launch_gemm<T, AX, BX, 256, 256, 128, 64, false>(g, s);
-    else rc = aligned ? launch_gemm<T, AX, BX, 128, 128, 64, 64, true>(g, s) : launch_gemm<T, AX, BX, 128, 128, 64, 64, false>(g, s);
+    else rc = aligned ? launch_gemm<T, AX, BX, 128, 128, 64, 32, true>(g, s) : launch_gemm<T, AX, BX, 128, 128, 64, 32, false>(g, s);
     if (rc) return rc;
     if (p.splits > 1) {
         const int64_t outs = a.rows * ((b.rows + 3) / 4);
