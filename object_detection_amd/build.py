@@ -1,4 +1,5 @@
-"""Builds object_detection_amd/libdetbox.so from csrc/*.hip with hipcc for gfx950.
+"""Builds object_detection_amd/libdetbox.so from csrc/*.hip with hipcc for gfx950, and object_detection_amd/_heads.so, the
+autograd nodes of the class-head operators, from csrc/heads.cpp with the host compiler and PyTorch's headers.
 
     python -m object_detection_amd.build [--force]
 
@@ -16,6 +17,9 @@ from concurrent.futures import ThreadPoolExecutor
 HERE = os.path.dirname(os.path.abspath(__file__))
 CSRC = os.path.join(HERE, 'csrc')
 OUT = os.path.join(HERE, 'libdetbox.so')
+HEADS_SRC = os.path.join(CSRC, 'heads.cpp')
+HEADS_OUT = os.path.join(HERE, '_heads.so')
+HEADER = os.path.join(HERE, '..', 'include', 'detbox.h')
 OBJ = os.path.join(HERE, 'csrc', '_obj')
 FLAGS = ['--offload-arch=gfx950', '-O3', '-std=c++17', '-fPIC', '-ffp-contract=off', '-Xclang', '-target-feature', '-Xclang',
          '-packed-fp32-ops', '-Wall', '-Wno-unused-function']
@@ -42,7 +46,29 @@ def needs_build():
     return any(os.path.getmtime(d) > os.path.getmtime(OUT) for d in deps)
 
 
+def heads_need_build():
+    return not os.path.exists(HEADS_OUT) or any(os.path.getmtime(d) > os.path.getmtime(HEADS_OUT) for d in (HEADS_SRC, HEADER))
+
+
+def build_heads(verbose=False):
+    """Host code only: it finds the entry points of libdetbox.so at run time."""
+    import sysconfig
+    import torch
+    from torch.utils import cpp_extension
+    torch_lib = os.path.join(os.path.dirname(torch.__file__), 'lib')
+    cmd = [os.environ.get('CXX', 'g++'), '-O2', '-std=c++17', '-fPIC', '-shared', '-Wall', '-Wno-unused-function',
+           '-D__HIP_PLATFORM_AMD__', '-DUSE_ROCM', '-D_GLIBCXX_USE_CXX11_ABI=%d' % int(torch._C._GLIBCXX_USE_CXX11_ABI)]
+    cmd += ['-isystem' + p for p in cpp_extension.include_paths('cuda') + [sysconfig.get_paths()['include']]]
+    cmd += [HEADS_SRC, '-o', HEADS_OUT, '-L' + torch_lib, '-Wl,-rpath,' + torch_lib, '-ltorch_python', '-ltorch', '-ltorch_cpu', '-lc10', '-lc10_hip']
+    if verbose:
+        print(' '.join(cmd))
+    subprocess.check_call(cmd)
+    return HEADS_OUT
+
+
 def build(force=False, verbose=False):
+    if force or heads_need_build():
+        build_heads(verbose)
     if not force and not needs_build():
         return OUT
     hipcc = os.environ.get('HIPCC', '/opt/rocm/bin/hipcc')

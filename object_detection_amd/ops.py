@@ -16,13 +16,13 @@ the host, and a missing library or GPU raises.
 """
 from __future__ import annotations
 
+import ctypes
 import os
 
 from dataclasses import dataclass
-from typing import List, Optional, Sequence, Tuple
+from typing import List, NamedTuple, Optional, Sequence, Tuple
 
 import torch
-from torch.autograd.function import once_differentiable
 
 from . import _lib
 
@@ -32,7 +32,6 @@ DECODE_CXCYWH, DECODE_YOLO, DECODE_FCOS = 0, 1, 2
 ACT_NONE, ACT_SOFTMAX, ACT_SOFTMAX_SIGMOID, ACT_SIGMOID_SIGMOID = 0, 1, 2, 3
 MAX_TOP_K = 4096
 NMS_MAX_SORT = 4096
-DTYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
 ACTIVATIONS = {'none': 0, 'relu': 1, 'gelu': 2, 'silu': 3, 'sigmoid': 4}
 MAX_ALTERNATIVES = 64
 
@@ -529,159 +528,28 @@ def pack_wire(boxes, scores, class_ids, keep, keep_counts, image_ids: torch.Tens
 
 # ------------------------------------------------------------------ class heads over many labels
 
-def _scratch(device, nbytes: int, tag: str, stream: int) -> Optional[torch.Tensor]:
-    """Workspace of a call that may be captured into a HIP graph: the cached buffer of _workspace in eager work; a buffer
-    of the graph's own while capturing, so that two graphs captured on one stream share none and a graph outlives any
-    growth of the cached one."""
-    if not nbytes:
-        return None
-    if not torch.cuda.is_current_stream_capturing():
-        return _workspace(device, nbytes, tag, stream)
-    ws = torch.empty(int(nbytes), dtype=torch.uint8, device=device)
-    if _POISON:
-        ws.fill_(0xA5)
-    return ws
+_heads_module = None
 
 
-def _rows(t: torch.Tensor) -> torch.Tensor:
-    """t as a matrix of its last axis: a view where the rows have one stride and unit element stride, a copy elsewhere
-    (expanded gradients, transposed inputs)."""
-    m = t.reshape(-1, t.shape[-1])
-    if (m.stride(1) == 1 or m.shape[1] == 1) and (m.shape[0] <= 1 or m.stride(0) >= m.shape[1]):
-        return m
-    return m.contiguous()
-
-
-def _ld(m: torch.Tensor) -> int:
-    return max(m.stride(0), m.shape[1]) if m.shape[0] > 1 else m.shape[1]
-
-
-def _head_input(name: str, what: str, t: torch.Tensor, device=None) -> None:
-    if not t.is_cuda:
-        raise _lib.DetboxError(f'{name} runs on a ROCm device only')
-    if device is not None and t.device != device:
-        raise ValueError(f'{name}: {what} is on {t.device}, not on {device}')
-    if t.dtype not in DTYPES:
-        raise ValueError(f'{name}: {what} is {t.dtype}; float32, bfloat16 and float16 are supported')
-
-
-def _wants_grad(*tensors) -> bool:
-    return torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors)
-
-
-def _layer_norm_forward(x, weight, bias, eps, keep):
-    dev = x.device
-    m = _rows(x)
-    rows, D = m.shape
-    param = weight if weight is not None else bias
-    pdt = DTYPES[param.dtype if param is not None else x.dtype]
-    weight = None if weight is None else weight.contiguous()
-    bias = None if bias is None else bias.contiguous()
-    y = torch.empty((rows, D), dtype=x.dtype, device=dev)
-    stats = torch.empty((rows, 2), dtype=torch.float32, device=dev) if keep else None
-    with _on(dev):
-        _lib.check(_lib.lib().detbox_layer_norm_forward(DTYPES[x.dtype], _ptr(m), _ld(m), pdt, _ptr(weight), _ptr(bias), rows, D, eps,
-                                                        _ptr(y), _ptr(stats), _stream(dev)), 'detbox_layer_norm_forward')
-    return y.view(x.shape), m, weight, stats, pdt
-
-
-class _LayerNorm(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, x, weight, bias, eps):
-        y, m, w, stats, pdt = _layer_norm_forward(x, weight, bias, eps, True)
-        ctx.save_for_backward(m, w, stats)
-        ctx.pdt, ctx.param_dtype, ctx.shape = pdt, None if weight is None and bias is None else (weight if weight is not None else bias).dtype, x.shape
-        return y
-
-    @staticmethod
-    @once_differentiable
-    def backward(ctx, grad):
-        m, weight, stats = ctx.saved_tensors
-        dev = m.device
-        rows, D = m.shape
-        g = _rows(grad)
-        gx = torch.empty((rows, D), dtype=m.dtype, device=dev) if ctx.needs_input_grad[0] else None
-        gw = torch.empty(D, dtype=ctx.param_dtype, device=dev) if ctx.needs_input_grad[1] else None
-        gb = torch.empty(D, dtype=ctx.param_dtype, device=dev) if ctx.needs_input_grad[2] else None
+def _heads():
+    """The native autograd nodes (csrc/heads.cpp), bound to the loaded library on first use."""
+    global _heads_module
+    if _heads_module is None:
         L = _lib.lib()
-        with _on(dev):
-            st = _stream(dev)
-            ws = _scratch(dev, _ws_bytes(dev, L.detbox_layer_norm_backward_workspace_bytes, rows, D), 'layer_norm', st)
-            _lib.check(L.detbox_layer_norm_backward(DTYPES[m.dtype], _ptr(g), _ld(g), _ptr(m), _ld(m), ctx.pdt, _ptr(weight), _ptr(stats),
-                                                    rows, D, _ptr(gx), _ptr(gw), _ptr(gb), _ptr(ws), 0 if ws is None else ws.numel(), st),
-                       'detbox_layer_norm_backward')
-        return None if gx is None else gx.view(ctx.shape), gw, gb, None
+        try:
+            from . import _heads as native
+        except ImportError as e:
+            raise _lib.DetboxError(f'the class-head operators are not built ({e}): build them with `python -m object_detection_amd.build`')
+        native.bind({n: ctypes.cast(getattr(L, n), ctypes.c_void_p).value for n in _lib.SIGNATURES}, _lib.DetboxError, _POISON)
+        _heads_module = native
+    return _heads_module
 
 
 def layer_norm(x: torch.Tensor, weight: Optional[torch.Tensor] = None, bias: Optional[torch.Tensor] = None,
                eps: float = 1e-5) -> torch.Tensor:
     """(x - mean) / sqrt(var + eps) * weight + bias over the last axis of x [..., D]; weight, bias [D] of one type (that of
     x or another of the three).  Differentiable in x, weight and bias; statistics and sums are fp32."""
-    _head_input('layer_norm', 'x', x)
-    if x.dim() < 1 or x.shape[-1] < 1:
-        raise ValueError('layer_norm: x needs a last axis of at least one element')
-    for what, p in (('weight', weight), ('bias', bias)):
-        if p is not None:
-            _head_input('layer_norm', what, p, x.device)
-            if p.shape != x.shape[-1:]:
-                raise ValueError(f'layer_norm: {what} {tuple(p.shape)} does not fit rows of {x.shape[-1]}')
-    if weight is not None and bias is not None and weight.dtype != bias.dtype:
-        raise ValueError('layer_norm: weight and bias differ in type')
-    if _wants_grad(x, weight, bias):
-        return _LayerNorm.apply(x, weight, bias, float(eps))
-    return _layer_norm_forward(x, weight, bias, float(eps), False)[0]
-
-
-def _linear_forward(x, weight, bias, act, residual, out_dtype, keep):
-    dev = x.device
-    m, w = _rows(x), _rows(weight)
-    (M, K), N = m.shape, w.shape[0]
-    bias = None if bias is None else bias.contiguous()
-    r = None if residual is None else _rows(residual)
-    y = torch.empty((M, N), dtype=out_dtype, device=dev)
-    pre = torch.empty((M, N), dtype=x.dtype, device=dev) if keep and act else None
-    L, dt = _lib.lib(), DTYPES[x.dtype]
-    with _on(dev):
-        st = _stream(dev)
-        ws = _scratch(dev, _ws_bytes(dev, L.detbox_linear_workspace_bytes, dt, M, N, K), 'linear', st)
-        _lib.check(L.detbox_linear_forward(dt, act, _ptr(m), _ld(m), _ptr(w), _ld(w), 0 if bias is None else DTYPES[bias.dtype],
-                                           _ptr(bias), _ptr(r), 0 if r is None else _ld(r), M, N, K, DTYPES[out_dtype], _ptr(y),
-                                           _ptr(pre), _ptr(ws), 0 if ws is None else ws.numel(), st), 'detbox_linear_forward')
-    return y.view(*x.shape[:-1], N), m, w, pre
-
-
-class _Linear(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, x, weight, bias, residual, act, out_dtype):
-        y, m, w, pre = _linear_forward(x, weight, bias, act, residual, out_dtype, any(ctx.needs_input_grad[:3]))
-        ctx.save_for_backward(m if ctx.needs_input_grad[1] else None, w if ctx.needs_input_grad[0] else None, pre)
-        ctx.act, ctx.x_shape, ctx.w_shape, ctx.dtype = act, x.shape, weight.shape, x.dtype
-        ctx.bias_dtype = None if bias is None else bias.dtype
-        return y
-
-    @staticmethod
-    @once_differentiable
-    def backward(ctx, grad):
-        m, w, pre = ctx.saved_tensors
-        need_x, need_w, need_b, need_r = ctx.needs_input_grad[:4]
-        dev = grad.device
-        gx = gw = gb = None
-        if need_x or need_w or need_b:
-            g = _rows(grad)
-            M, (N, K) = g.shape[0], ctx.w_shape
-            gx = torch.empty((M, K), dtype=ctx.dtype, device=dev) if need_x else None
-            gw = torch.empty((N, K), dtype=ctx.dtype, device=dev) if need_w else None
-            gb = torch.empty(N, dtype=ctx.bias_dtype, device=dev) if need_b else None
-            L, dt, gdt = _lib.lib(), DTYPES[ctx.dtype], DTYPES[g.dtype]
-            with _on(dev):
-                st = _stream(dev)
-                ws = _scratch(dev, _ws_bytes(dev, L.detbox_linear_backward_workspace_bytes, dt, ctx.act, gdt, M, N, K), 'linear', st)
-                _lib.check(L.detbox_linear_backward(dt, ctx.act, gdt, _ptr(g), _ld(g), _ptr(pre), _ptr(m), K if m is None else _ld(m), _ptr(w),
-                                                    K if w is None else _ld(w), M, N, K, _ptr(gx), _ptr(gw),
-                                                    0 if gb is None else DTYPES[gb.dtype], _ptr(gb), _ptr(ws),
-                                                    0 if ws is None else ws.numel(), st), 'detbox_linear_backward')
-            gx = None if gx is None else gx.view(ctx.x_shape)
-        return gx, gw, gb, grad if need_r else None, None, None
+    return _heads().layer_norm(x, weight, bias, eps)
 
 
 def linear(x: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Tensor] = None, activation: str = 'none',
@@ -691,88 +559,18 @@ def linear(x: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Tensor] =
     out_dtype=torch.float32, the fp32 sum itself (the logits select_decode and focal_loss_sum take).  Differentiable in x,
     weight, bias and residual; products are summed in fp32, the gradient at the activation's input is rounded to the type
     of x before it is multiplied."""
-    _head_input('linear', 'x', x)
-    _head_input('linear', 'weight', weight, x.device)
-    if activation not in ACTIVATIONS:
+    act = ACTIVATIONS.get(activation)
+    if act is None:
         raise ValueError(f'linear: unknown activation {activation!r}')
-    if weight.dim() != 2 or x.dim() < 1 or weight.shape[1] != x.shape[-1] or weight.shape[0] < 1 or weight.shape[1] < 1:
-        raise ValueError(f'linear: x {tuple(x.shape)} and weight {tuple(weight.shape)} do not fit')
-    if weight.dtype != x.dtype:
-        raise ValueError('linear: x and weight differ in type')
-    out_dtype = x.dtype if out_dtype is None else out_dtype
-    if out_dtype not in (x.dtype, torch.float32):
-        raise ValueError(f'linear: out_dtype {out_dtype} is neither the type of x nor float32')
-    if bias is not None:
-        _head_input('linear', 'bias', bias, x.device)
-        if bias.shape != weight.shape[:1]:
-            raise ValueError(f'linear: bias {tuple(bias.shape)} does not fit weight {tuple(weight.shape)}')
-    if residual is not None:
-        _head_input('linear', 'residual', residual, x.device)
-        if residual.shape != (*x.shape[:-1], weight.shape[0]) or residual.dtype != out_dtype:
-            raise ValueError(f'linear: residual {tuple(residual.shape)} of {residual.dtype} does not fit the output')
-    if _wants_grad(x, weight, bias, residual):
-        return _Linear.apply(x, weight, bias, residual, ACTIVATIONS[activation], out_dtype)
-    return _linear_forward(x, weight, bias, ACTIVATIONS[activation], residual, out_dtype, False)[0]
+    return _heads().linear(x, weight, bias, act, residual, out_dtype)
 
 
-@dataclass
-class LabelLogProbs:
+class LabelLogProbs(NamedTuple):
     """Output of label_log_probs; every tensor has the leading axes of the logits."""
     log_probs: torch.Tensor                    # [...] fp32: log probability of the row's label (0 where the label is ignored)
     entropy: Optional[torch.Tensor]            # [...] fp32, or None
     top_log_probs: Optional[torch.Tensor]      # [..., top_k] fp32 in descending order, or None
     top_ids: Optional[torch.Tensor]            # [..., top_k] int64, or None
-
-
-def _label_log_probs_forward(logits, labels, top_k, entropy, keep):
-    dev = logits.device
-    m = _rows(logits)
-    rows, C = m.shape
-    t = labels.reshape(-1).to(torch.int64).contiguous()
-    lp = torch.empty(rows, dtype=torch.float32, device=dev)
-    ent = torch.empty(rows, dtype=torch.float32, device=dev) if entropy else None
-    tv = torch.empty((rows, top_k), dtype=torch.float32, device=dev) if top_k else None
-    ti = torch.empty((rows, top_k), dtype=torch.int64, device=dev) if top_k else None
-    stats = torch.empty((rows, 2), dtype=torch.float32, device=dev) if keep else None
-    L = _lib.lib()
-    with _on(dev):
-        st = _stream(dev)
-        ws = _scratch(dev, _ws_bytes(dev, L.detbox_label_log_probs_workspace_bytes, rows, C, top_k), 'label_log_probs', st)
-        _lib.check(L.detbox_label_log_probs_forward(DTYPES[m.dtype], _ptr(m), _ld(m), _ptr(t), rows, C, top_k, _ptr(lp), _ptr(ent),
-                                                    _ptr(tv), _ptr(ti), _ptr(stats), _ptr(ws), 0 if ws is None else ws.numel(), st),
-                   'detbox_label_log_probs_forward')
-    shape = logits.shape[:-1]
-    return (lp.view(shape), None if ent is None else ent.view(shape), None if tv is None else tv.view(*shape, top_k),
-            None if ti is None else ti.view(*shape, top_k), m, t, stats)
-
-
-class _LabelLogProbs(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, logits, labels, top_k, entropy):
-        lp, ent, tv, ti, m, t, stats = _label_log_probs_forward(logits, labels, top_k, entropy, True)
-        ctx.save_for_backward(m, t, stats, ent)
-        ctx.shape = logits.shape
-        ctx.set_materialize_grads(False)
-        if top_k:
-            ctx.mark_non_differentiable(tv, ti)
-        return lp, ent, tv, ti
-
-    @staticmethod
-    @once_differentiable
-    def backward(ctx, grad_lp, grad_ent, *_):
-        m, t, stats, ent = ctx.saved_tensors
-        if grad_lp is None and grad_ent is None:
-            return None, None, None, None
-        dev = m.device
-        rows, C = m.shape
-        g = None if grad_lp is None else grad_lp.reshape(-1).contiguous()
-        h = None if grad_ent is None else grad_ent.reshape(-1).contiguous()
-        gx = torch.empty((rows, C), dtype=m.dtype, device=dev)
-        with _on(dev):
-            _lib.check(_lib.lib().detbox_label_log_probs_backward(DTYPES[m.dtype], _ptr(m), _ld(m), _ptr(t), rows, C, _ptr(stats),
-                                                                  _ptr(ent), _ptr(g), _ptr(h), _ptr(gx), _stream(dev)),
-                       'detbox_label_log_probs_backward')
-        return gx.view(ctx.shape), None, None, None
 
 
 def label_log_probs(logits: torch.Tensor, labels: torch.Tensor, top_k: int = 0, entropy: bool = False) -> LabelLogProbs:
@@ -782,19 +580,7 @@ def label_log_probs(logits: torch.Tensor, labels: torch.Tensor, top_k: int = 0, 
     negative labels of focal_loss_sum.  Differentiable in `logits` through log_probs and entropy; the alternatives are
     not differentiable.  A logit of -inf is a class that cannot be; a row of -inf only has log probability -inf, entropy
     0 and gradient 0."""
-    _head_input('label_log_probs', 'logits', logits)
-    if logits.dim() < 1 or logits.shape[-1] < 1:
-        raise ValueError('label_log_probs: logits need a last axis of at least one class')
-    if labels.device != logits.device:
-        raise ValueError(f'label_log_probs: labels are on {labels.device}, not on {logits.device}')
-    if labels.shape != logits.shape[:-1] or labels.is_floating_point() or labels.is_complex() or labels.dtype is torch.bool:
-        raise ValueError(f'label_log_probs: labels {tuple(labels.shape)} of {labels.dtype} do not fit logits {tuple(logits.shape)}')
-    top_k = int(top_k)
-    if not 0 <= top_k <= min(MAX_ALTERNATIVES, logits.shape[-1]):
-        raise ValueError(f'label_log_probs: top_k {top_k} is outside 0 .. min({MAX_ALTERNATIVES}, {logits.shape[-1]})')
-    if _wants_grad(logits):
-        return LabelLogProbs(*_LabelLogProbs.apply(logits, labels, top_k, bool(entropy)))
-    return LabelLogProbs(*_label_log_probs_forward(logits, labels, top_k, bool(entropy), False)[:4])
+    return LabelLogProbs(*_heads().label_log_probs(logits, labels, int(top_k), bool(entropy), MAX_ALTERNATIVES))
 
 
 def topk_mask(values: torch.Tensor, k: torch.Tensor) -> torch.Tensor:
