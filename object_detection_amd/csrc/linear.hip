@@ -129,15 +129,17 @@ __device__ inline void store4(void *p, int dtype, int64_t i, int n, f32x4 v) {
     for (int j = 0; j < n; ++j) store_from_float(p, dtype, i + j, v[j]);
 }
 
-// Four neighbouring sums of row m, columns n .. n + 3 (those below N), through the epilogue.
-__device__ inline void finish4(const Epilogue &ep, int64_t m, int64_t n, int64_t N, f32x4 z) {
-    const int left = N - n < 4 ? (int)(N - n) : 4;
+// Four neighbouring sums of a row, columns n .. n + 3 (those below N), through the epilogue.  `row` is the row's offset in the
+// outputs, `res_row` that in the residual: kept by the caller, since a 64-bit product per four elements costs more than
+// everything else here.
+__device__ inline void finish4(const Epilogue &ep, int64_t row, int64_t res_row, int n, int N, f32x4 z) {
+    const int left = N - n < 4 ? N - n : 4;
     if (left <= 0) return;
     if (ep.bias) z += load4(ep.bias, ep.bias_dtype, n, left);
-    if (ep.pre) store4(ep.pre, ep.pre_dtype, m * N + n, left, z);
+    if (ep.pre) store4(ep.pre, ep.pre_dtype, row + n, left, z);
     if (ep.act != DETBOX_ACTIVATION_NONE) z = act4(z, ep.act);
-    if (ep.residual) z += load4(ep.residual, ep.out_dtype, m * ep.ldr + n, left);
-    store4(ep.out, ep.out_dtype, m * N + n, left, z);
+    if (ep.residual) z += load4(ep.residual, ep.out_dtype, res_row + n, left);
+    store4(ep.out, ep.out_dtype, row + n, left, z);
 }
 
 // ---- tile kernel ---------------------------------------------------------------------------------------------------------
@@ -262,9 +264,11 @@ __device__ inline detbox_u4 read_fragment(const char *lds, int row0, int ks) {
     }
 }
 
-// acc[n = 4 (l / 16) + i][m = l % 16] += sum over the fragments' contraction
+// acc[n = 4 (l / 16) + i][m = l % 16] += sum over part `t` of the fragments' contraction: all of it for the 16-bit types, a
+// quarter for fp32, whose instruction takes one element per lane.
+template <typename T> constexpr int PARTS = sizeof(T) == 2 ? 1 : 4;
 template <typename T>
-__device__ inline f32x4 multiply(detbox_u4 n, detbox_u4 m, f32x4 acc) {
+__device__ inline f32x4 multiply(detbox_u4 n, detbox_u4 m, f32x4 acc, int t) {
     if constexpr (std::is_same_v<T, __bf16>) {
         typedef __bf16 v8 __attribute__((ext_vector_type(8)));
         return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(v8, n), __builtin_bit_cast(v8, m), acc, 0, 0, 0);
@@ -272,19 +276,18 @@ __device__ inline f32x4 multiply(detbox_u4 n, detbox_u4 m, f32x4 acc) {
         typedef _Float16 v8 __attribute__((ext_vector_type(8)));
         return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(v8, n), __builtin_bit_cast(v8, m), acc, 0, 0, 0);
     } else {
-        const f32x4 a = __builtin_bit_cast(f32x4, n), b = __builtin_bit_cast(f32x4, m);
-#pragma unroll
-        for (int j = 0; j < 4; ++j) acc = __builtin_amdgcn_mfma_f32_16x16x4f32(a[j], b[j], acc, 0, 0, 0);
-        return acc;
+        return __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(n[t]), __uint_as_float(m[t]), acc, 0, 0, 0);
     }
 }
 
-// Workgroups are dealt to the eight XCDs in turn.  Every XCD gets a run of neighbouring tiles, walked in bands of eight tile
-// rows, so that the operands' panels are shared in its L2.
-__device__ inline void tile_of(int wg, int tiles_m, int tiles_n, int &tm, int &tn) {
-    const int total = tiles_m * tiles_n, per = total / 8, rest = total % 8;
+// Workgroups are dealt to the eight XCDs in turn.  Every XCD gets a run of neighbouring jobs, so that the operands' panels are
+// shared in its L2: the tiles of one piece of the contraction one after the other, walked in bands of eight tile rows.
+__device__ inline void job_of(int wg, int tiles_m, int tiles_n, int splits, int &tm, int &tn, int &split) {
+    const int tiles = tiles_m * tiles_n, total = tiles * splits, per = total / 8, rest = total % 8;
     const int x = wg & 7, i = wg >> 3;
-    const int t = x * per + (x < rest ? x : rest) + i;
+    const int job = x * per + (x < rest ? x : rest) + i;
+    split = job / tiles;
+    const int t = job - split * tiles;
     const int band = t / (8 * tiles_n), rows = tiles_m - band * 8 < 8 ? tiles_m - band * 8 : 8;
     const int in = t - band * 8 * tiles_n;
     tm = band * 8 + in % rows;
@@ -306,9 +309,11 @@ __device__ __forceinline__ void multiply_step(const char *__restrict__ cur, int 
 #pragma unroll
         for (int j = 0; j < FN; ++j) fb[j] = read_fragment<T, BX, BN>(cur + BM * 128, wn + j * 16, ks);
 #pragma unroll
-        for (int i = 0; i < FM; ++i)
+        for (int t = 0; t < PARTS<T>; ++t)                     // neighbouring instructions add to different sums
 #pragma unroll
-            for (int j = 0; j < FN; ++j) acc[i][j] = multiply<T>(fb[j], fa[i], acc[i][j]);
+            for (int i = 0; i < FM; ++i)
+#pragma unroll
+                for (int j = 0; j < FN; ++j) acc[i][j] = multiply<T>(fb[j], fa[i], acc[i][j], t);
     }
     if constexpr (sizeof(T) == 2) {
         constexpr int READS = FM * (AX ? 2 : 1) + FN * (BX ? 2 : 1), EACH = FM * FN / READS;
@@ -340,10 +345,9 @@ __global__ __launch_bounds__((BM / WM) * (BN / WN) * 64) void gemm_kernel(GemmAr
     extern __shared__ __attribute__((aligned(16))) char lds[];
     const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
     const int wm = (wave % (BM / WM)) * WM, wn = (wave / (BM / WM)) * WN;
-    int tm, tn;
-    tile_of(blockIdx.x, g.tiles_m, g.tiles_n, tm, tn);
+    int tm, tn, split;
+    job_of(blockIdx.x, g.tiles_m, g.tiles_n, g.splits, tm, tn, split);
     const int64_t m0 = (int64_t)tm * BM, n0 = (int64_t)tn * BN;
-    const int split = blockIdx.y;
     const int64_t s0 = split * g.steps_per_split, all = (g.K + STEP_K<T> - 1) / STEP_K<T>;
     const int64_t steps = all - s0 < g.steps_per_split ? all - s0 : g.steps_per_split;
 
@@ -421,12 +425,13 @@ __global__ __launch_bounds__((BM / WM) * (BN / WN) * 64) void gemm_kernel(GemmAr
         __builtin_amdgcn_wave_barrier();
         // a batch of rows at a time: the residual's loads of a batch are on their way together
         constexpr int TURNS = (HALF + AT_ONCE - 1) / AT_ONCE, U = TURNS < 8 ? TURNS : 8;
+        const int64_t row0 = m0 + wm + h * HALF + lane / LANES, out_at = row0 * N + n, res_at = row0 * g.ep.ldr + n;
         for (int t = 0; t < TURNS; t += U) {
             detbox_u4 raw[U];
             auto row_of = [&](int u) { return (t + u) * AT_ONCE + lane / LANES; };
             auto alive = [&](int u) { return row_of(u) < HALF && m0 + wm + h * HALF + row_of(u) < M; };
             if (g.ep.residual && left == 4) {
-                const int64_t at = (m0 + wm + h * HALF + row_of(0)) * g.ep.ldr + n, by = (int64_t)AT_ONCE * g.ep.ldr;
+                const int64_t at = res_at + (int64_t)t * AT_ONCE * g.ep.ldr, by = (int64_t)AT_ONCE * g.ep.ldr;
                 if (g.ep.out_dtype == DETBOX_F32) {
 #pragma unroll
                     for (int u = 0; u < U; ++u)
@@ -444,17 +449,19 @@ __global__ __launch_bounds__((BM / WM) * (BN / WN) * 64) void gemm_kernel(GemmAr
 #pragma unroll
             for (int u = 0; u < U; ++u) {
                 if (left <= 0 || !alive(u)) continue;
-                const int64_t m = m0 + wm + h * HALF + row_of(u);
                 f32x4 z = *reinterpret_cast<const f32x4 *>(mine + row_of(u) * ROW + (lane % LANES) * 4);
+                const int64_t at = out_at + (int64_t)((t + u) * AT_ONCE) * N;
                 if (g.splits > 1) {
-                    store4(g.part, DETBOX_F32, ((int64_t)split * M + m) * N + n, left, z);
+                    store4(g.part, DETBOX_F32, (int64_t)split * M * N + at, left, z);
                     continue;
                 }
                 z += bias;
-                if (g.ep.pre) store4(g.ep.pre, g.ep.pre_dtype, m * N + n, left, z);
+                if (g.ep.pre) store4(g.ep.pre, g.ep.pre_dtype, at, left, z);
                 if (g.ep.act != DETBOX_ACTIVATION_NONE) z = act4(z, g.ep.act);
-                if (g.ep.residual) z += left == 4 ? widen4(raw[u], g.ep.out_dtype) : load4(g.ep.residual, g.ep.out_dtype, m * g.ep.ldr + n, left);
-                store4(g.ep.out, g.ep.out_dtype, m * N + n, left, z);
+                if (g.ep.residual)
+                    z += left == 4 ? widen4(raw[u], g.ep.out_dtype)
+                                   : load4(g.ep.residual, g.ep.out_dtype, res_at + (int64_t)((t + u) * AT_ONCE) * g.ep.ldr, left);
+                store4(g.ep.out, g.ep.out_dtype, at, left, z);
             }
         }
     }
@@ -485,12 +492,12 @@ __global__ __launch_bounds__(256) void gemm_join_kernel(const float *__restrict_
             }
             __syncthreads();
         }
-        if (slice == 0 && left > 0) finish4(ep, m, n, N, z);
+        if (slice == 0 && left > 0) finish4(ep, m * N, m * ep.ldr, (int)n, (int)N, z);
     }
 }
 
 // dz = g * act'(pre) in the type of x with rows of ldz elements (zeros behind N), and partial column sums of the unrounded dz
-// per row slice.  LANES lanes share a row, four columns each; HBM bound.
+// per row slice.  LANES lanes share a row, four columns each; HBM bound (16384 x 4096 bf16 with gelu: 96 us = 4.2 TB/s).
 template <typename T, int LANES>
 __global__ __launch_bounds__(256) void linear_slope_kernel(const void *g, int gdt, int64_t ldg, const T *__restrict__ pre, int act,
                                                            int64_t M, int64_t N, int64_t ldz, int64_t rows_per_slice,
@@ -502,11 +509,13 @@ __global__ __launch_bounds__(256) void linear_slope_kernel(const void *g, int gd
     f32x4 a = {0.f, 0.f, 0.f, 0.f};
     const int64_t lo = blockIdx.y * rows_per_slice, hi = lo + rows_per_slice < M ? lo + rows_per_slice : M;
     if (c < ldz) {
-#pragma unroll 2
-        for (int64_t row = lo + threadIdx.x / LANES; row < hi; row += ROWS) {
-            f32x4 v = load4(g, gdt, row * ldg + c, left);
-            if (pre) v *= slope4(load4(pre, DT, row * N + c, left), act);          // v is 0 behind N
-            if (dz) store4(dz, DT, row * ldz + c, room, v);
+        const int64_t row0 = lo + threadIdx.x / LANES, by_g = ROWS * ldg, by_p = ROWS * N, by_z = ROWS * ldz;
+        int64_t at_g = row0 * ldg + c, at_p = row0 * N + c, at_z = row0 * ldz + c;
+#pragma unroll 1                                                              // more waves hide more than rows in flight do: 96 us against 131 unrolled
+        for (int64_t row = row0; row < hi; row += ROWS, at_g += by_g, at_p += by_p, at_z += by_z) {
+            f32x4 v = load4(g, gdt, at_g, left);
+            if (pre) v *= slope4(load4(pre, DT, at_p, left), act);                // v is 0 behind N
+            if (dz) store4(dz, DT, at_z, room, v);
             a += v;
         }
     }
@@ -526,17 +535,18 @@ __global__ __launch_bounds__(256) void linear_slope_kernel(const void *g, int gd
 // waves stream rows of A straight into registers, 16 MF at a time, each on its own: no barrier after the set-up, and what
 // bounds it is the read of A and the write of C.  RetinaNet's class logits (480348 x 256 bf16 by 81, fp32 out): 202 us with
 // tiles of 256 x 256 that drain their pipeline every four steps, 89 us = 4.5 TB/s so.
-constexpr int RES_BLOCK = 512, RES_LDS = 128 * 1024;
+constexpr int RES_LDS = 128 * 1024;
+template <int NF> constexpr int RES_BLOCK = NF > 6 ? 512 : 1024;         // one workgroup per CU: 16 waves as far as registers go
 
 template <typename T, bool BX, int MF, int NF>
-__global__ __launch_bounds__(RES_BLOCK, NF > 6 ? 2 : 4) void gemm_resident_kernel(const Operand<T> a, const Operand<T> b, int64_t K,
+__global__ __launch_bounds__(RES_BLOCK<NF>, NF > 6 ? 2 : 4) void gemm_resident_kernel(const Operand<T> a, const Operand<T> b, int64_t K,
                                                                                  int groups, Epilogue ep) {
     constexpr int VEC = VEC_OF<T>, KF = 4 * VEC, CHUNK = 8 / MF > 4 ? 8 : 4;       // contraction of one fragment; fragments in flight
     extern __shared__ __attribute__((aligned(16))) char lds[];
     const int lane = threadIdx.x & 63, r = lane & 15, q = lane >> 4;
     const int64_t M = a.rows, N = b.rows;
     const int kf = (int)((K + KF - 1) / KF), all = groups * NF;
-    for (int i = threadIdx.x; i < kf * all * 64; i += RES_BLOCK) {
+    for (int i = threadIdx.x; i < kf * all * 64; i += RES_BLOCK<NF>) {
         const int f = i >> 6, l = i & 63;
         const int64_t n = (f % all) * 16 + (l & 15), k = (int64_t)(f / all) * KF + (l >> 4) * VEC;
         detbox_u4 u = {0, 0, 0, 0};
@@ -555,8 +565,8 @@ __global__ __launch_bounds__(RES_BLOCK, NF > 6 ? 2 : 4) void gemm_resident_kerne
         *reinterpret_cast<detbox_u4 *>(lds + i * 16) = u;
     }
     __syncthreads();
-    const int64_t blocks = (M + 16 * MF - 1) / (16 * MF), waves = (int64_t)gridDim.x * (RES_BLOCK / 64);
-    for (int64_t rb = (int64_t)blockIdx.x * (RES_BLOCK / 64) + (threadIdx.x >> 6); rb < blocks; rb += waves) {
+    const int64_t blocks = (M + 16 * MF - 1) / (16 * MF), waves = (int64_t)gridDim.x * (RES_BLOCK<NF> / 64);
+    for (int64_t rb = (int64_t)blockIdx.x * (RES_BLOCK<NF> / 64) + (threadIdx.x >> 6); rb < blocks; rb += waves) {
         const T *row[MF];
 #pragma unroll
         for (int i = 0; i < MF; ++i) {
@@ -600,20 +610,24 @@ __global__ __launch_bounds__(RES_BLOCK, NF > 6 ? 2 : 4) void gemm_resident_kerne
                 for (int c = 0; c < CHUNK; ++c) {
                     if (c0 + c >= kf) break;
                     const char *at = lds + (((c0 + c) * all + g * NF) * 64 + own) * 16;
+                    detbox_u4 fb[NF];
 #pragma unroll
-                    for (int j = 0; j < NF; ++j) {
-                        const detbox_u4 fb = *reinterpret_cast<const detbox_u4 *>(at + j * 1024);
+                    for (int j = 0; j < NF; ++j) fb[j] = *reinterpret_cast<const detbox_u4 *>(at + j * 1024);
 #pragma unroll
-                        for (int i = 0; i < MF; ++i) acc[i][j] = multiply<T>(fb, fa[c][i], acc[i][j]);
-                    }
+                    for (int t = 0; t < PARTS<T>; ++t)
+#pragma unroll
+                        for (int j = 0; j < NF; ++j)
+#pragma unroll
+                            for (int i = 0; i < MF; ++i) acc[i][j] = multiply<T>(fb[j], fa[c][i], acc[i][j], t);
                 }
             }
 #pragma unroll
             for (int i = 0; i < MF; ++i) {
                 const int64_t m = rb * 16 * MF + i * 16 + r;
                 if (m < M) {
+                    const int64_t at = m * N, res = m * ep.ldr;
 #pragma unroll
-                    for (int j = 0; j < NF; ++j) finish4(ep, m, (g * NF + j) * 16 + quarter * 4, N, acc[i][j]);
+                    for (int j = 0; j < NF; ++j) finish4(ep, at, res, (g * NF + j) * 16 + quarter * 4, (int)N, acc[i][j]);
                 }
             }
         }
@@ -664,7 +678,7 @@ int launch_gemm(const GemmArgs<T> &g, hipStream_t s) {
     constexpr int BUFFERS = 2 * (BM + BN) * 128, OUT = WAVES * HALF * (WN + 4) * 4, LDS = BUFFERS > OUT ? BUFFERS : OUT;
     auto kernel = gemm_kernel<T, AX, BX, BM, BN, WM, WN, ALIGNED>;
     DETBOX_HIP(hipFuncSetAttribute(reinterpret_cast<const void *>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, LDS));
-    kernel<<<dim3((unsigned)(g.tiles_m * g.tiles_n), (unsigned)g.splits), dim3(WAVES * 64), LDS, s>>>(g);
+    kernel<<<dim3((unsigned)(g.tiles_m * g.tiles_n * g.splits)), dim3(WAVES * 64), LDS, s>>>(g);
     DETBOX_LAUNCH_CHECK();
     return DETBOX_OK;
 }
@@ -686,9 +700,8 @@ int launch_resident(const Operand<T> &a, const Operand<T> &b, int64_t K, const E
     const int all = resident_columns(b.rows), lds = (int)((K + KF - 1) / KF * all * 1024);
     auto kernel = gemm_resident_kernel<T, BX, MF, NF>;
     DETBOX_HIP(hipFuncSetAttribute(reinterpret_cast<const void *>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, RES_LDS));
-    const int64_t blocks = (a.rows + 16 * MF - 1) / (16 * MF), wgs = (blocks + RES_BLOCK / 64 - 1) / (RES_BLOCK / 64);
-    const int64_t most = lds > 80 * 1024 || NF > 6 ? 256 : 512;         // one or two per CU
-    kernel<<<dim3((unsigned)(wgs < most ? wgs : most)), dim3(RES_BLOCK), lds, s>>>(a, b, K, all / NF, ep);
+    const int64_t blocks = (a.rows + 16 * MF - 1) / (16 * MF), wgs = (blocks + RES_BLOCK<NF> / 64 - 1) / (RES_BLOCK<NF> / 64);
+    kernel<<<dim3((unsigned)(wgs < 256 ? wgs : 256)), dim3(RES_BLOCK<NF>), lds, s>>>(a, b, K, all / NF, ep);
     DETBOX_LAUNCH_CHECK();
     return DETBOX_OK;
 }
@@ -696,7 +709,7 @@ template <typename T, bool BX>
 int gemm_resident(const Operand<T> &a, const Operand<T> &b, int64_t K, const Epilogue &ep, hipStream_t s) {
     if (b.rows <= 32) return launch_resident<T, BX, 2, 2>(a, b, K, ep, s);
     if (b.rows <= 64) return launch_resident<T, BX, 2, 4>(a, b, K, ep, s);
-    if (b.rows <= 96) return launch_resident<T, BX, 2, 6>(a, b, K, ep, s);
+    if (b.rows <= 96) return launch_resident<T, BX, 1, 6>(a, b, K, ep, s);
     return launch_resident<T, BX, 2, 8>(a, b, K, ep, s);
 }
 
