@@ -634,6 +634,74 @@ __global__ __launch_bounds__(RES_BLOCK<NF>, NF > 6 ? 2 : 4) void gemm_resident_k
     }
 }
 
+// ---- few rows ------------------------------------------------------------------------------------------------------------
+
+// At most 16 MT rows of x (serving): the weight is all there is to read, and it goes straight into registers, once.  A workgroup
+// owns 16 columns; its eight waves take the contraction's packs in turn and add their sums in LDS in order.  No second launch.
+// 4 x 4096 by 4096 bf16 with everything in the epilogue: 13.7 us as tiles in pieces and their join, 9.2 us = 3.7 TB/s so.
+constexpr int64_t FEW_ROWS = 64;
+constexpr int FEW_BLOCK = 512, FEW_WAVES = FEW_BLOCK / 64;
+
+template <typename T, int MT>
+__global__ __launch_bounds__(FEW_BLOCK) void gemm_few_kernel(const Operand<T> a, const Operand<T> b, int64_t K, Epilogue ep) {
+    constexpr int VEC = VEC_OF<T>, KF = 4 * VEC, CHUNK = MT > 2 ? 4 : 8;
+    __shared__ f32x4 sums[FEW_WAVES][MT][64];
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, r = lane & 15, q = lane >> 4;
+    const int64_t M = a.rows, N = b.rows, kf = (K + KF - 1) / KF;
+    for (int64_t n0 = (int64_t)blockIdx.x * 16; n0 < N; n0 += (int64_t)gridDim.x * 16) {
+        const int64_t n = n0 + r < N ? n0 + r : N - 1;                       // columns and rows that do not exist: any values
+        const T *w = b.p + n * b.ld, *x[MT];
+#pragma unroll
+        for (int i = 0; i < MT; ++i) x[i] = a.p + (i * 16 + r < M ? i * 16 + r : M - 1) * a.ld;
+        f32x4 acc[MT];
+#pragma unroll
+        for (int i = 0; i < MT; ++i) acc[i] = f32x4{0.f, 0.f, 0.f, 0.f};
+        int64_t c0 = wave;
+        for (; (c0 + (CHUNK - 1) * FEW_WAVES + 1) * KF <= K; c0 += FEW_WAVES * CHUNK) {
+            detbox_u4 fw[CHUNK], fx[CHUNK][MT];
+#pragma unroll
+            for (int c = 0; c < CHUNK; ++c) {
+                const int64_t k = (c0 + c * FEW_WAVES) * KF + q * VEC;
+                fw[c] = load_raw_nt<T>(w + k);
+#pragma unroll
+                for (int i = 0; i < MT; ++i) fx[c][i] = load_raw<T>(x[i] + k);
+            }
+#pragma unroll
+            for (int c = 0; c < CHUNK; ++c)
+#pragma unroll
+                for (int t = 0; t < PARTS<T>; ++t)
+#pragma unroll
+                    for (int i = 0; i < MT; ++i) acc[i] = multiply<T>(fw[c], fx[c][i], acc[i], t);
+        }
+        for (; c0 < kf; c0 += FEW_WAVES) {                                  // the rest, the row's last pack moved down to its place
+            const int64_t k = c0 * KF + q * VEC, over = k + VEC - K, at = over <= 0 ? k : K - VEC;     // K >= VEC here
+            detbox_u4 fw = load_raw_nt<T>(w + at), fx[MT];
+#pragma unroll
+            for (int i = 0; i < MT; ++i) fx[i] = load_raw<T>(x[i] + at);
+            if (over > 0) {
+                fw = moved_down<T>(fw, over);
+#pragma unroll
+                for (int i = 0; i < MT; ++i) fx[i] = moved_down<T>(fx[i], over);
+            }
+#pragma unroll
+            for (int t = 0; t < PARTS<T>; ++t)
+#pragma unroll
+                for (int i = 0; i < MT; ++i) acc[i] = multiply<T>(fw, fx[i], acc[i], t);
+        }
+#pragma unroll
+        for (int i = 0; i < MT; ++i) sums[wave][i][lane] = acc[i];
+        __syncthreads();
+        if (wave < MT) {
+            f32x4 z = sums[0][wave][lane];
+#pragma unroll
+            for (int v = 1; v < FEW_WAVES; ++v) z += sums[v][wave][lane];
+            const int64_t m = wave * 16 + r;
+            if (m < M) finish4(ep, m * N, m * ep.ldr, (int)n0 + q * 4, (int)N, z);
+        }
+        __syncthreads();
+    }
+}
+
 // ---- host ----------------------------------------------------------------------------------------------------------------
 
 bool act_ok(int act) { return act >= DETBOX_ACTIVATION_NONE && act <= DETBOX_ACTIVATION_SIGMOID; }
@@ -713,10 +781,33 @@ int gemm_resident(const Operand<T> &a, const Operand<T> &b, int64_t K, const Epi
     return launch_resident<T, BX, 2, 8>(a, b, K, ep, s);
 }
 
+// Measured in bf16 against the tiles (us): 1 x 1000 by 1203 4.5 / 9.9, 64 x 1000 by 1203 6.2 / 12.4, 1 x 4096 by 4096 7.6 / 11.5,
+// 16 rows of it 11.7 / 12.9, 32 rows 15.5 / 15.0; with more to read, where every workgroup's copy of x counts, the tiles lead
+// (64 x 4096 by 4096 22.7 / 18.6, 1 x 4096 by 32000 56 / 41), and so they do where a long contraction is eight waves' only
+// (64 x 4096 by 81 20 / 10).
+bool few(int dtype, int64_t M, int64_t N, int64_t K) {
+    const int64_t vec = 16 / (int64_t)dtype_size(dtype), tiles = (M + 15) / 16, kf = (K + 4 * vec - 1) / (4 * vec);
+    return M <= FEW_ROWS && K >= vec && tiles * N * K <= 20 << 20 && kf <= (tiles > 2 ? 64 : 256);
+}
+
+template <typename T>
+int gemm_few(const Operand<T> &a, const Operand<T> &b, int64_t K, const Epilogue &ep, hipStream_t s) {
+    const int64_t columns = (b.rows + 15) / 16;
+    const dim3 grid((unsigned)(columns < 1 << 20 ? columns : 1 << 20)), block(FEW_BLOCK);
+    if (a.rows <= 16) gemm_few_kernel<T, 1><<<grid, block, 0, s>>>(a, b, K, ep);
+    else if (a.rows <= 32) gemm_few_kernel<T, 2><<<grid, block, 0, s>>>(a, b, K, ep);
+    else gemm_few_kernel<T, 4><<<grid, block, 0, s>>>(a, b, K, ep);
+    DETBOX_LAUNCH_CHECK();
+    return DETBOX_OK;
+}
+
 template <typename T, bool AX, bool BX>
 int gemm(const Operand<T> &a, const Operand<T> &b, int64_t K, int dtype, const Epilogue &ep, void *workspace, hipStream_t s) {
     if constexpr (!AX) {
         if (resident(dtype, a.rows, b.rows, K)) return gemm_resident<T, BX>(a, b, K, ep, s);
+    }
+    if constexpr (!AX && !BX) {
+        if (few(dtype, a.rows, b.rows, K)) return gemm_few<T>(a, b, K, ep, s);
     }
     const Plan p = plan_of(dtype, a.rows, b.rows, K);
     const GemmArgs<T> g{a, b, K, p.tiles_m, p.tiles_n, p.splits, p.steps_per_split, ep, static_cast<float *>(workspace)};
@@ -765,7 +856,7 @@ Slices slices_of(int64_t M, int64_t N) {
 
 extern "C" size_t detbox_linear_workspace_bytes(int dtype, int64_t M, int64_t N, int64_t K) {
     if (!dtype_ok(dtype) || M < 1 || N < 1 || K < 1) return 0;
-    return plan_bytes(plan_of(dtype, M, N, K), M, N);
+    return few(dtype, M, N, K) || resident(dtype, M, N, K) ? 0 : plan_bytes(plan_of(dtype, M, N, K), M, N);
 }
 
 extern "C" int detbox_linear_forward(int dtype, int activation, const void *x, int64_t ldx, const void *weight, int64_t ldw,

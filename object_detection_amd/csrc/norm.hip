@@ -3,7 +3,7 @@
 //   gw = g * w:  grad_x = r * (gw - mean(gw) - h * mean(gw * h)),  grad_w = sum over rows of g * h,  grad_b = sum of g
 // All statistics and sums are fp32; every output is rounded once.
 //
-// HBM bound.  A row lives in the registers of a group of 4, 16, 64, 256 or 1024 lanes, 8 or 16 elements each, so that it is
+// HBM bound.  A row lives in the registers of a group of 4, 16, 64, 256, 512 or 1024 lanes, 8 or 16 elements each, so that it is
 // read once and the deviations are squared about the mean itself.  A lane keeps the parameters of its columns, and in the
 // backward pass their gradients, in registers over all the rows its group takes; the groups' sums meet in LDS, the
 // workgroups' in the workspace.  Rows of more than 16384 elements are walked three times.
@@ -261,7 +261,7 @@ __global__ __launch_bounds__(NORM_BLOCK) void norm_long_columns_kernel(const T *
 int64_t at_most(int64_t v, int64_t most) { return v < most ? v : most; }
 
 // Lanes per row for rows of D <= LONG_ROW elements: the group of 16 elements per lane that holds them.
-int lanes_of(int64_t D) { return D <= 64 ? 4 : D <= 256 ? 16 : D <= 1024 ? 64 : D <= 4096 ? 256 : 1024; }
+int lanes_of(int64_t D) { return D <= 64 ? 4 : D <= 256 ? 16 : D <= 1024 ? 64 : D <= 4096 ? 256 : D <= 8192 ? 512 : 1024; }
 
 // Workgroups of the backward pass, each of which leaves one row of partial sums: four per CU, one of 1024 threads.
 int workgroups_of(int64_t rows, int64_t D) {
@@ -291,6 +291,7 @@ void with_group(int64_t D, F &&fn) {
             if (D <= 2048) call(integral_constant<int, 256>{}, integral_constant<int, W>{});
             else call(integral_constant<int, 256>{}, integral_constant<int, 2 * W>{});
             break;
+        case 512: call(integral_constant<int, 512>{}, integral_constant<int, 2 * W>{}); break;
         default: call(integral_constant<int, 1024>{}, integral_constant<int, 2 * W>{});
     }
 }
