@@ -172,6 +172,7 @@ int detbox_smooth_l1_masked_backward(const float *input, const float *target, co
 #define DETBOX_ACTIVATION_SIGMOID 4
 
 #define DETBOX_MAX_ALTERNATIVES 64  /* largest top_k of detbox_label_log_probs_forward */
+#define DETBOX_LINEAR_MAX_TILES (1ll << 23) /* M x N, M x K and N x K each hold fewer tiles of 128 x 128 */
 
 /* y = (x - mean) / sqrt(var + eps) * weight + bias over rows of D elements (var: the mean of the squared deviations).
  *   weight, bias  [D] of param_dtype, each may be NULL

@@ -76,9 +76,14 @@ void check_input(const char *name, const char *what, const Tensor &t, const Tens
         refuse(name, ": ", what, " is ", t.scalar_type(), "; float32, bfloat16 and float16 are supported");
 }
 
-// Runs in autograd's threads as well: a plain C++ exception, which arrives in Python as RuntimeError.
+// Called with Python's lock held (a forward call) an error of the library is the package's DetboxError, like everywhere else;
+// in autograd's threads it is a C++ exception, which arrives in Python as RuntimeError, DetboxError's base.
 void check(int rc, const char *what) {
-    if (rc) throw std::runtime_error(c10::str(what, " failed with code ", rc, ": ", api.last_error()));
+    if (!rc) return;
+    const std::string text = c10::str(what, " failed with code ", rc, ": ", api.last_error());
+    if (!PyGILState_Check()) throw std::runtime_error(text);
+    PyErr_SetString(device_error, text.c_str());
+    throw py::error_already_set();
 }
 
 // ---- layout, streams, scratch --------------------------------------------------------------------------------------------

@@ -832,7 +832,10 @@ int check_linear(int dtype, int act, int64_t ldx, int64_t ldw, int64_t M, int64_
     DETBOX_CHECK_ARG(ldx >= K && ldw >= K, "row stride below the row length");
     // tiles are counted in 32 bits in each of the three products
     auto tiles = [](int64_t a, int64_t b) { return ((a + 127) / 128) * ((b + 127) / 128); };
-    DETBOX_CHECK_ARG(tiles(M, N) < (1ll << 23) && tiles(M, K) < (1ll << 23) && tiles(N, K) < (1ll << 23), "size too large");
+    if (tiles(M, N) >= DETBOX_LINEAR_MAX_TILES || tiles(M, K) >= DETBOX_LINEAR_MAX_TILES || tiles(N, K) >= DETBOX_LINEAR_MAX_TILES) {
+        set_error("%s: a product of DETBOX_LINEAR_MAX_TILES tiles or more", __func__);
+        return DETBOX_ERR_UNSUPPORTED;
+    }
     return DETBOX_OK;
 }
 

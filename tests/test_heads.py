@@ -240,6 +240,25 @@ def test_linear(dtype, M, N, K):
     check_linear(x, w, b, None, 'none', torch.float32, gr.float(), 'fp32 out')
 
 
+# many rows against few columns (whole weight on chip), and products that fill the chip with large tiles; each with rows that
+# start at multiples of 16 bytes and without
+@pytest.mark.gpu
+@pytest.mark.parametrize('dtype', TYPES, ids=str)
+@pytest.mark.parametrize('M,N,K', [(32768, 81, 256), (33001, 20, 37), (33001, 64, 300), (32769, 97, 61), (98304, 200, 24), (98311, 301, 31),
+                                   (3584, 3712, 3600), (3600, 3700, 3650)])
+def test_linear_large(dtype, M, N, K):
+    g = torch.Generator(device='cuda').manual_seed(M + N + K)
+
+    def rand(*shape, dtype=dtype, scale=1.0):
+        return (torch.randn(*shape, generator=g, device='cuda') * scale).to(dtype)
+    x, w, b, r, gr = rand(M, K), rand(N, K, scale=K ** -0.5), rand(N), rand(M, N), rand(M, N)
+    check_linear(x, w, b, r, 'gelu', None, gr, 'gelu')
+    check_linear(x, w, None, r.float(), 'relu', torch.float32, gr.float(), 'relu, fp32 out')
+    check_linear(x, w, b, None, 'none', None, gr, 'plain')
+    wide = torch.cat([rand(M, 3), x], 1)
+    check_linear(wide[:, 3:], w, b, None, 'silu', None, gr, 'off alignment')
+
+
 @pytest.mark.gpu
 @pytest.mark.parametrize('dtype', TYPES, ids=str)
 @pytest.mark.parametrize('M', [1, 5, 90])
@@ -266,7 +285,8 @@ def test_linear_whole_values(dtype):
     """Whole numbers whose products and sums every type holds: the result is exact, so no element, column or split of the
     long axis is lost, doubled or misplaced; with more rows than one round of tiles and a long contraction."""
     g = gen(9)
-    for M, N, K in ((1, 300, 4096), (7, 130, 1000), (64, 64, 64), (530, 270, 200), (3000, 19, 24), (2, 2, 9000), (1040, 512, 520)):
+    for M, N, K in ((1, 300, 4096), (7, 130, 1000), (64, 64, 64), (530, 270, 200), (3000, 19, 24), (2, 2, 9000), (1040, 512, 520), (33000, 24, 64), (98400, 300, 24),
+                    (3600, 3700, 1000)):
         x = torch.randint(-1, 2, (M, K), generator=g).to(dtype).to('cuda').requires_grad_()
         w = (torch.randint(-1, 2, (N, K), generator=g) * (torch.rand(N, K, generator=g) < 100.0 / K)).to(dtype).to('cuda').requires_grad_()
         gr = (torch.randint(-1, 2, (M, N), generator=g) * (torch.rand(M, N, generator=g) < min(1.0, 100.0 / max(M, N)))).to(dtype).to('cuda')
@@ -678,6 +698,60 @@ def test_refusals():
         torch.autograd.grad(gx.sum(), x)
 
 
+@pytest.mark.gpu
+def test_offsets_beyond_32_bits():
+    """Operands of more than 2^32 elements: the last rows give what the same rows give alone."""
+    t = torch.bfloat16
+    g = gen(18)
+
+    def tail_of(rows, n, k):
+        big = torch.zeros(rows, n, dtype=t, device='cuda')
+        assert big.numel() > 2 ** 32
+        big[-k:] = randn(g, k, n, dtype=t)
+        return big.requires_grad_(), big[-k:].detach().clone().requires_grad_()
+    k = 40
+    # logits: 33000 rows of 131072
+    x, small = tail_of(33000, 131072, k)
+    labels = torch.randint(0, 131072, (33000,), generator=g).cuda()
+    a, b = ops.label_log_probs(x, labels, 3, True), ops.label_log_probs(small, labels[-k:], 3, True)
+    assert torch.equal(a.top_ids[-k:], b.top_ids)
+    for u, v in ((a.log_probs[-k:], b.log_probs), (a.entropy[-k:], b.entropy)):
+        assert torch.allclose(u, v, rtol=1e-5, atol=0)              # rows cut into pieces or not: the sums' order differs
+    gr = randn(g, 33000)
+    (gx,), (gs,) = torch.autograd.grad(a.log_probs, x, gr), torch.autograd.grad(b.log_probs, small, gr[-k:])
+    assert float((gx[-k:].float() - gs.float()).norm()) <= 2.0 ** -8 * float(gs.float().norm())
+    # rows of zeros: -g / C everywhere but at the label, whose g (1 - 1 / C) is of another size
+    head = gx[:3].detach().float().scatter(1, labels[:3].clamp(min=0)[:, None], 0.0).abs().amax(1)
+    assert torch.all(head <= gr[:3].abs() / 131072 * (1 + 2.0 ** -7))
+    del x, gx, a
+    # rows for a norm and a product: 1100000 of 4096
+    x, small = tail_of(1100000, 4096, k)
+    w, b = randn(g, 4096, dtype=t), randn(g, 4096, dtype=t)
+    y, ys = ops.layer_norm(x, w, b), ops.layer_norm(small, w, b)
+    assert torch.equal(y[-k:], ys)
+    gr = torch.zeros_like(x)
+    gr[-k:] = randn(g, k, 4096, dtype=t)
+    gx, gs = torch.autograd.grad(y, x, gr)[0], torch.autograd.grad(ys, small, gr[-k:])[0]
+    assert torch.equal(gx[-k:], gs) and not gx[:100].any()
+    del y, gx, gr
+    w = randn(g, 24, 4096, dtype=t, scale=1 / 64).requires_grad_()
+    y, ys = ops.linear(x, w), ops.linear(small, w)
+    # both are within one rounding of the same sums, taken in another order
+    assert torch.allclose(y[-k:].float(), ys.float(), rtol=2.0 ** -7, atol=2.0 ** -10) and not y[:100].any()
+    gr = torch.zeros_like(y)
+    gr[-k:] = randn(g, k, 24, dtype=t)
+    (gx, gw), (gs, gv) = torch.autograd.grad(y, [x, w], gr), torch.autograd.grad(ys, [small, w], gr[-k:])
+    for u, v in ((gx[-k:], gs), (gw, gv)):
+        assert torch.allclose(u.float(), v.float(), rtol=2.0 ** -7, atol=2.0 ** -8)
+
+
+@pytest.mark.gpu
+def test_library_errors_are_the_packages():
+    """A limit of the library arrives as DetboxError."""
+    with pytest.raises(_lib.DetboxError, match='DETBOX_LINEAR_MAX_TILES'):
+        ops.linear(torch.zeros(1 << 30, 1, dtype=torch.float16, device='cuda'), torch.zeros(1, 1, dtype=torch.float16, device='cuda'))
+
+
 def test_refuse_without_a_device():
     x = torch.zeros(2, 3)
     for call in (lambda: ops.layer_norm(x), lambda: ops.linear(x, x), lambda: ops.label_log_probs(x, torch.zeros(2, dtype=torch.int64))):
@@ -709,6 +783,13 @@ def test_c_entry_points_refuse():
     assert L.detbox_linear_forward(0, 0, p, 8, p, 8, 0, None, p, 3, 2, 4, 8, 0, p, None, None, 0, None) == inv
     assert L.detbox_linear_forward(0, 0, p, 8, None, 8, 0, None, None, 0, 2, 4, 8, 0, p, None, None, 0, None) == inv
     assert L.detbox_linear_forward(0, 0, None, 8, None, 8, 0, None, None, 0, 0, 4, 8, 0, None, None, None, 0, None) == 0
+    assert L.detbox_linear_forward(0, 0, p, 8, p, 8, 0, None, None, 0, 1 << 30, 4, 8, 0, p, None, None, 0, None) == unsup
+    need = L.detbox_linear_workspace_bytes(1, 300, 4096, 4096)
+    assert need >= 300 * 4096 * 4
+    assert L.detbox_linear_forward(1, 0, p, 4096, p, 4096, 0, None, None, 0, 300, 4096, 4096, 1, p, None, p, need - 1, None) == ws_err
+    need = L.detbox_label_log_probs_workspace_bytes(1, 100000, 4)
+    assert need > 0
+    assert L.detbox_label_log_probs_forward(0, p, 100000, p, 1, 100000, 4, p, None, p, p, None, p, need - 1, None) == ws_err
     need = L.detbox_linear_backward_workspace_bytes(1, 2, 1, 100, 40, 24)
     assert need >= 100 * 40 * 2
     assert L.detbox_linear_backward(1, 2, 1, p, 40, p, p, 24, p, 24, 100, 40, 24, p, p, 0, p, p, need - 1, None) == ws_err
