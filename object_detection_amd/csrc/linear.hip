@@ -5,6 +5,10 @@
 // there is an activation) and the z that the derivative is taken at; both are operands of the same matrix instructions as
 // x and W, which have that type.
 //
+// Bounds: a long contraction is bound by the matrix instructions (8192^3 bf16 1.25-1.31 PFLOP/s in all three products), a short
+// one by memory (RetinaNet's class logits, 480348 x 256 bf16 by 81, fp32 out: 88 us = 3.7 TB/s), few rows by the read of the
+// weight (4 x 4096 by 4096: 9 us = 3.7 TB/s).
+//
 // One tile kernel serves all three products.  Each operand lies in memory either along the contraction (x, W forward) or
 // across it (W in grad_x; dz and x in grad_W); both come into LDS as they lie, 16 bytes at a time, and only the read of a
 // fragment differs: a plain 16-byte read, or the transposing LDS read of 16-bit elements.
@@ -166,9 +170,10 @@ template <typename T> constexpr int STEP_K = 128 / (int)sizeof(T);
 // Where the chunks of a step lie in LDS.  Along: chunk c of row r at slot c ^ (r & 7) of the row's 128 bytes, so that the 16
 // rows a fragment read touches spread over all banks.  Across: rows of the contraction, each ROWS elements in units of 16
 // (one fragment's width); unit u of row k at u ^ swizzle(k), which spreads the rows that one read touches.
-template <typename T>
+template <typename T, int ROWS>
 __device__ inline int across_swizzle(int k) {
-    return sizeof(T) == 2 ? (k & 3) | ((k >> 3) & 1) << 2 : (k >> 2) & 3;
+    static_assert((ROWS & (ROWS - 1)) == 0, "units are swapped in powers of two");
+    return (sizeof(T) == 2 ? (k & 3) | ((k >> 3) & 1) << 2 : (k >> 2) & 3) & (ROWS / 16 - 1);
 }
 
 __device__ const uint4 zero_chunk = {0, 0, 0, 0};
@@ -176,11 +181,14 @@ __device__ const uint4 zero_chunk = {0, 0, 0, 0};
 // The chunks of one step that a thread brings in: idx = j * THREADS + tid is also the place in LDS.
 template <typename T, bool ACROSS, int ROWS, int THREADS, bool ALIGNED>
 struct Stager {
-    static constexpr int VEC = VEC_OF<T>, COUNT = ROWS * 8 / THREADS, PER_K = ROWS / VEC, PER_UNIT = 16 / VEC;
+    static constexpr int VEC = VEC_OF<T>, COUNT = (ROWS * 8 + THREADS - 1) / THREADS, PER_K = ROWS / VEC, PER_UNIT = 16 / VEC;
     const T *src[COUNT];        // of the step that is fetched next
     int at[COUNT];              // contraction index of the chunk inside a step
     int left[COUNT];            // across: how many of the chunk's elements exist
     int64_t step;               // elements from one step to the next
+
+    // Whether there is a chunk j for this thread: whole waves have one or not.
+    static __device__ bool live(int j) { return ROWS * 8 % THREADS == 0 || j * THREADS + (int)(threadIdx.x & ~63) < ROWS * 8; }
 
     __device__ void init(const Operand<T> &o, int64_t row0, int64_t k0) {
         const int tid = threadIdx.x;
@@ -188,9 +196,9 @@ struct Stager {
 #pragma unroll
         for (int j = 0; j < COUNT; ++j) {
             const int idx = j * THREADS + tid;
-            if (ACROSS) {
+            if constexpr (ACROSS) {
                 const int k = idx / PER_K, slot = idx % PER_K;
-                const int unit = (slot / PER_UNIT) ^ across_swizzle<T>(k);
+                const int unit = (slot / PER_UNIT) ^ across_swizzle<T, ROWS>(k);
                 int64_t r = row0 + unit * 16 + (slot % PER_UNIT) * VEC;
                 at[j] = k;
                 const int64_t n = o.extent - r;
@@ -210,6 +218,7 @@ struct Stager {
     }
     // Brings chunk j of the next step straight into LDS (aligned operands; chunks behind the contraction's end from a zero).
     __device__ void dma(int j, int64_t k_left, char *lds) {
+        if (!live(j)) return;
         const void *p = src[j];
         src[j] += step;
         if (k_left < STEP_K<T> && at[j] >= k_left) p = &zero_chunk;
@@ -217,6 +226,7 @@ struct Stager {
     }
     // Chunk j of the next step, which starts k_left elements before the contraction's end; zeros behind the end.
     __device__ detbox_u4 load(int j, int64_t k_left) {
+        if (!live(j)) return detbox_u4{0, 0, 0, 0};
         const T *p = src[j];
         src[j] = p + step;
         int n = left[j];
@@ -236,16 +246,15 @@ struct Stager {
 template <typename T, bool ACROSS, int ROWS>
 __device__ inline detbox_u4 read_fragment(const char *lds, int row0, int ks) {
     const int lane = threadIdx.x & 63, r = lane & 15, q = lane >> 4;
-    if (!ACROSS) {
+    if constexpr (!ACROSS) {
         const int row = row0 + r;
         return *reinterpret_cast<const detbox_u4 *>(lds + (row * 8 + ((ks * 4 + q) ^ (row & 7))) * 16);
-    }
-    if constexpr (sizeof(T) == 2) {
+    } else if constexpr (sizeof(T) == 2) {
         detbox_u4 u;
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
             const int k = ks * 32 + q * 8 + h * 4 + (r >> 2);
-            const char *p = lds + k * (ROWS * 2) + (((row0 >> 4) ^ across_swizzle<T>(k)) * 32) + (r & 3) * 8;
+            const char *p = lds + k * (ROWS * 2) + (((row0 >> 4) ^ across_swizzle<T, ROWS>(k)) * 32) + (r & 3) * 8;
             const s16x4 v = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4 *)p);
             typedef uint32_t u2 __attribute__((ext_vector_type(2)));
             const u2 w = __builtin_bit_cast(u2, v);
@@ -258,7 +267,7 @@ __device__ inline detbox_u4 read_fragment(const char *lds, int row0, int ks) {
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
             const int k = ks * 16 + q * 4 + j;
-            u[j] = *reinterpret_cast<const uint32_t *>(lds + k * (ROWS * 4) + (((row0 >> 4) ^ across_swizzle<T>(k)) * 64) + r * 4);
+            u[j] = *reinterpret_cast<const uint32_t *>(lds + k * (ROWS * 4) + (((row0 >> 4) ^ across_swizzle<T, ROWS>(k)) * 64) + r * 4);
         }
         return u;
     }
@@ -315,8 +324,8 @@ __device__ __forceinline__ void multiply_step(const char *__restrict__ cur, int 
 #pragma unroll
                 for (int j = 0; j < FN; ++j) acc[i][j] = multiply<T>(fb[j], fa[i], acc[i][j], t);
     }
-    if constexpr (sizeof(T) == 2) {
-        constexpr int READS = FM * (AX ? 2 : 1) + FN * (BX ? 2 : 1), EACH = FM * FN / READS;
+    constexpr int READS = FM * (AX ? 2 : 1) + FN * (BX ? 2 : 1), EACH = FM * FN / READS;
+    if constexpr (sizeof(T) == 2 && EACH > 0) {
         __builtin_amdgcn_sched_group_barrier(0x100, READS, 0);
 #pragma unroll
         for (int r = 0; r < READS; ++r) {
@@ -391,9 +400,11 @@ __global__ __launch_bounds__((BM / WM) * (BN / WN) * 64) void gemm_kernel(GemmAr
         };
         auto put = [&](char *to) {
 #pragma unroll
-            for (int j = 0; j < sa.COUNT; ++j) *reinterpret_cast<detbox_u4 *>(to + (j * THREADS + threadIdx.x) * 16) = ra[j];
+            for (int j = 0; j < sa.COUNT; ++j)
+                if (sa.live(j)) *reinterpret_cast<detbox_u4 *>(to + (j * THREADS + threadIdx.x) * 16) = ra[j];
 #pragma unroll
-            for (int j = 0; j < sb.COUNT; ++j) *reinterpret_cast<detbox_u4 *>(to + A_BYTES + (j * THREADS + threadIdx.x) * 16) = rb[j];
+            for (int j = 0; j < sb.COUNT; ++j)
+                if (sb.live(j)) *reinterpret_cast<detbox_u4 *>(to + A_BYTES + (j * THREADS + threadIdx.x) * 16) = rb[j];
         };
         if (steps > 0) {
             fetch(0);
@@ -529,116 +540,11 @@ __global__ __launch_bounds__(256) void linear_slope_kernel(const void *g, int gd
     }
 }
 
-// ---- many rows against few columns -----------------------------------------------------------------------------------------
-
-// B (all columns, the whole contraction) stays in LDS for the workgroup's life, in the order in which fragments are read; the
-// waves stream rows of A straight into registers, 16 MF at a time, each on its own: no barrier after the set-up, and what
-// bounds it is the read of A and the write of C.  RetinaNet's class logits (480348 x 256 bf16 by 81, fp32 out): 202 us with
-// tiles of 256 x 256 that drain their pipeline every four steps, 89 us = 4.5 TB/s so.
-constexpr int RES_LDS = 128 * 1024;
-template <int NF> constexpr int RES_BLOCK = NF > 6 ? 512 : 1024;         // one workgroup per CU: 16 waves as far as registers go
-
-template <typename T, bool BX, int MF, int NF>
-__global__ __launch_bounds__(RES_BLOCK<NF>, NF > 6 ? 2 : 4) void gemm_resident_kernel(const Operand<T> a, const Operand<T> b, int64_t K,
-                                                                                 int groups, Epilogue ep) {
-    constexpr int VEC = VEC_OF<T>, KF = 4 * VEC, CHUNK = 8 / MF > 4 ? 8 : 4;       // contraction of one fragment; fragments in flight
-    extern __shared__ __attribute__((aligned(16))) char lds[];
-    const int lane = threadIdx.x & 63, r = lane & 15, q = lane >> 4;
-    const int64_t M = a.rows, N = b.rows;
-    const int kf = (int)((K + KF - 1) / KF), all = groups * NF;
-    for (int i = threadIdx.x; i < kf * all * 64; i += RES_BLOCK<NF>) {
-        const int f = i >> 6, l = i & 63;
-        const int64_t n = (f % all) * 16 + (l & 15), k = (int64_t)(f / all) * KF + (l >> 4) * VEC;
-        detbox_u4 u = {0, 0, 0, 0};
-        if (BX) {
-            T e[VEC];
-#pragma unroll
-            for (int j = 0; j < VEC; ++j) e[j] = b.p[(k + j < K ? k + j : K - 1) * b.ld + (n < N ? n : N - 1)];
-#pragma unroll
-            for (int j = 0; j < VEC; ++j)
-                if (n >= N || k + j >= K) e[j] = (T)0.f;
-            __builtin_memcpy(&u, e, 16);
-        } else if (n < N && k < K) {
-            u = load_raw<T>(b.p + n * b.ld + (k + VEC <= K ? k : K - VEC));
-            if (k + VEC > K) u = moved_down<T>(u, k + VEC - K);
-        }
-        *reinterpret_cast<detbox_u4 *>(lds + i * 16) = u;
-    }
-    __syncthreads();
-    const int64_t blocks = (M + 16 * MF - 1) / (16 * MF), waves = (int64_t)gridDim.x * (RES_BLOCK<NF> / 64);
-    for (int64_t rb = (int64_t)blockIdx.x * (RES_BLOCK<NF> / 64) + (threadIdx.x >> 6); rb < blocks; rb += waves) {
-        const T *row[MF];
-#pragma unroll
-        for (int i = 0; i < MF; ++i) {
-            int64_t m = rb * 16 * MF + i * 16 + r;
-            m = m < M ? m : M - 1;                              // rows that do not exist: any values
-            row[i] = a.p + m * a.ld;
-        }
-        detbox_u4 fa[CHUNK][MF];
-        for (int g = 0; g < groups; ++g) {
-            // Opaque copies: what depends on the lane only would otherwise be computed once for every fragment and kept, some
-            // hundred registers of it.
-            int own = lane, quarter = q;
-            asm volatile("" : "+v"(own), "+v"(quarter));
-            f32x4 acc[MF][NF];
-#pragma unroll
-            for (int i = 0; i < MF; ++i)
-#pragma unroll
-                for (int j = 0; j < NF; ++j) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
-            for (int c0 = 0; c0 < kf; c0 += CHUNK) {
-                if (g == 0 || kf > CHUNK) {                              // a short contraction's rows are kept for all groups
-#pragma unroll
-                    for (int c = 0; c < CHUNK; ++c)
-#pragma unroll
-                        for (int i = 0; i < MF; ++i) {
-                            const int64_t k = (int64_t)(c0 + c) * KF + quarter * VEC;
-                            // the last whole pack where the row ends earlier; K >= VEC here
-                            fa[c][i] = load_raw_nt<T>(row[i] + (k + VEC <= K ? k : K - VEC));
-                        }
-                    if ((int64_t)(c0 + CHUNK) * KF > K) {
-#pragma unroll
-                        for (int c = 0; c < CHUNK; ++c) {
-                            const int64_t k = (int64_t)(c0 + c) * KF + quarter * VEC;
-                            if (k + VEC > K) {
-#pragma unroll
-                                for (int i = 0; i < MF; ++i) fa[c][i] = moved_down<T>(fa[c][i], k + VEC - K);
-                            }
-                        }
-                    }
-                }
-#pragma unroll
-                for (int c = 0; c < CHUNK; ++c) {
-                    if (c0 + c >= kf) break;
-                    const char *at = lds + (((c0 + c) * all + g * NF) * 64 + own) * 16;
-                    detbox_u4 fb[NF];
-#pragma unroll
-                    for (int j = 0; j < NF; ++j) fb[j] = *reinterpret_cast<const detbox_u4 *>(at + j * 1024);
-#pragma unroll
-                    for (int t = 0; t < PARTS<T>; ++t)
-#pragma unroll
-                        for (int j = 0; j < NF; ++j)
-#pragma unroll
-                            for (int i = 0; i < MF; ++i) acc[i][j] = multiply<T>(fb[j], fa[c][i], acc[i][j], t);
-                }
-            }
-#pragma unroll
-            for (int i = 0; i < MF; ++i) {
-                const int64_t m = rb * 16 * MF + i * 16 + r;
-                if (m < M) {
-                    const int64_t at = m * N, res = m * ep.ldr;
-#pragma unroll
-                    for (int j = 0; j < NF; ++j) finish4(ep, at, res, (g * NF + j) * 16 + quarter * 4, (int)N, acc[i][j]);
-                }
-            }
-        }
-    }
-}
-
 // ---- few rows ------------------------------------------------------------------------------------------------------------
 
 // At most 16 MT rows of x (serving): the weight is all there is to read, and it goes straight into registers, once.  A workgroup
 // owns 16 columns; its eight waves take the contraction's packs in turn and add their sums in LDS in order.  No second launch.
-// 4 x 4096 by 4096 bf16 with everything in the epilogue: 13.7 us as tiles in pieces and their join, 9.2 us = 3.7 TB/s so.
+// 4 x 4096 by 4096 bf16: 11.1 us as tiles in pieces and their join, 9.2 us = 3.7 TB/s so.
 constexpr int64_t FEW_ROWS = 64;
 constexpr int FEW_BLOCK = 512, FEW_WAVES = FEW_BLOCK / 64;
 
@@ -707,18 +613,20 @@ __global__ __launch_bounds__(FEW_BLOCK) void gemm_few_kernel(const Operand<T> a,
 bool act_ok(int act) { return act >= DETBOX_ACTIVATION_NONE && act <= DETBOX_ACTIVATION_SIGMOID; }
 
 // How a product is cut.  Tiles of 256 x 256 (eight waves of 128 x 64, one workgroup per CU) where they alone fill the chip and
-// have steps enough to hide their start and end; tiles of 128 x 128 (eight waves of 64 x 32, two workgroups per CU)
-// otherwise, with the contraction in pieces where there are fewer than two tiles per CU.  Measured (bf16, us, large / small):
-// 8192^3 860 / 1043, 4096^3 115 / 132, 8192 x 1024 by 8192 149 / 153, 8192 x 512 by 8192 103 / 95, 65536 x 256 by 256
-// 24 / 21, 2048^3 (64 large tiles) 59 / 31.
-struct Plan { bool big; int tiles_m, tiles_n, splits; int64_t steps_per_split; };
-Plan plan_of(int dtype, int64_t M, int64_t N, int64_t K) {
+// have steps enough to hide their start and end; tiles of 128 rows (eight waves, two or three workgroups per CU) otherwise,
+// as wide as the columns ask for, with the contraction in pieces where there are fewer than two tiles per CU.  Measured (bf16
+// unless it says fp32, us, large / small): 8192^3 860 / 1043, 4096^3 115 / 132, 8192 x 1024 by 8192 149 / 153, 8192 x 512 by
+// 8192 103 / 95, 65536 x 256 by 256 24 / 21, 2048^3 (64 large tiles) 59 / 31.  Width (128 / as wide as needed): 480348 x 64 by
+// 32 39 / 22, 40000 x 300 by 20 11.7 / 8.6, 120087 x 256 by 81 in fp32, where the matrix instructions count, 87 / 71.
+struct Plan { bool big; int width, tiles_m, tiles_n, splits; int64_t steps_per_split; };
+Plan plan_of(int dtype, int64_t M, int64_t N, int64_t K, bool across) {
     Plan p;
     const int64_t step = 128 / (int64_t)dtype_size(dtype), steps = (K + step - 1) / step;
     p.big = ((M + 255) / 256) * ((N + 255) / 256) >= 192 && steps > 8;
     const int64_t t = p.big ? 256 : 128;
+    p.width = p.big ? 256 : N <= 64 ? 64 : N <= 96 && !across ? 96 : 128;
     p.tiles_m = (int)((M + t - 1) / t);
-    p.tiles_n = (int)((N + t - 1) / t);
+    p.tiles_n = (int)((N + p.width - 1) / p.width);
     int64_t splits = 1;
     if (!p.big) {
         splits = 512 / ((int64_t)p.tiles_m * p.tiles_n);
@@ -751,36 +659,6 @@ int launch_gemm(const GemmArgs<T> &g, hipStream_t s) {
     return DETBOX_OK;
 }
 
-// Whether B fits LDS whole (128 KB) and there are rows enough to pay for bringing it there.  Measured in bf16 against the tiles
-// (us): 32768 x 512 by 128 22 / 33, 16384 x 256 by 81 13 / 13, 8192 x 1024 by 32 22 / 12; with more columns it only pays
-// where a short contraction leaves the tiles' pipeline no steps: 120087 x 64 by 512 55 / 64, 32768 x 64 by 512 30 / 19,
-// 120087 x 256 by 256 74 / 45.
-int resident_columns(int64_t N) { return (int)(N <= 32 ? 2 : N <= 64 ? 4 : N <= 96 ? 6 : (N + 127) / 128 * 8); }
-bool resident(int dtype, int64_t M, int64_t N, int64_t K) {
-    const int64_t vec = 16 / (int64_t)dtype_size(dtype), kf = (K + 4 * vec - 1) / (4 * vec);
-    if (K < vec || N > 512 || kf * resident_columns(N) * 1024 > RES_LDS) return false;
-    return N <= 128 ? M >= 32768 : M >= 98304 && K * (int64_t)dtype_size(dtype) <= 256;
-}
-
-template <typename T, bool BX, int MF, int NF>
-int launch_resident(const Operand<T> &a, const Operand<T> &b, int64_t K, const Epilogue &ep, hipStream_t s) {
-    constexpr int64_t KF = 4 * VEC_OF<T>;
-    const int all = resident_columns(b.rows), lds = (int)((K + KF - 1) / KF * all * 1024);
-    auto kernel = gemm_resident_kernel<T, BX, MF, NF>;
-    DETBOX_HIP(hipFuncSetAttribute(reinterpret_cast<const void *>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, RES_LDS));
-    const int64_t blocks = (a.rows + 16 * MF - 1) / (16 * MF), wgs = (blocks + RES_BLOCK<NF> / 64 - 1) / (RES_BLOCK<NF> / 64);
-    kernel<<<dim3((unsigned)(wgs < 256 ? wgs : 256)), dim3(RES_BLOCK<NF>), lds, s>>>(a, b, K, all / NF, ep);
-    DETBOX_LAUNCH_CHECK();
-    return DETBOX_OK;
-}
-template <typename T, bool BX>
-int gemm_resident(const Operand<T> &a, const Operand<T> &b, int64_t K, const Epilogue &ep, hipStream_t s) {
-    if (b.rows <= 32) return launch_resident<T, BX, 2, 2>(a, b, K, ep, s);
-    if (b.rows <= 64) return launch_resident<T, BX, 2, 4>(a, b, K, ep, s);
-    if (b.rows <= 96) return launch_resident<T, BX, 1, 6>(a, b, K, ep, s);
-    return launch_resident<T, BX, 2, 8>(a, b, K, ep, s);
-}
-
 // Measured in bf16 against the tiles (us): 1 x 1000 by 1203 4.5 / 9.9, 64 x 1000 by 1203 6.2 / 12.4, 1 x 4096 by 4096 7.6 / 11.5,
 // 16 rows of it 11.7 / 12.9, 32 rows 15.5 / 15.0; with more to read, where every workgroup's copy of x counts, the tiles lead
 // (64 x 4096 by 4096 22.7 / 18.6, 1 x 4096 by 32000 56 / 41), and so they do where a long contraction is eight waves' only
@@ -803,18 +681,22 @@ int gemm_few(const Operand<T> &a, const Operand<T> &b, int64_t K, const Epilogue
 
 template <typename T, bool AX, bool BX>
 int gemm(const Operand<T> &a, const Operand<T> &b, int64_t K, int dtype, const Epilogue &ep, void *workspace, hipStream_t s) {
-    if constexpr (!AX) {
-        if (resident(dtype, a.rows, b.rows, K)) return gemm_resident<T, BX>(a, b, K, ep, s);
-    }
     if constexpr (!AX && !BX) {
         if (few(dtype, a.rows, b.rows, K)) return gemm_few<T>(a, b, K, ep, s);
     }
-    const Plan p = plan_of(dtype, a.rows, b.rows, K);
+    const Plan p = plan_of(dtype, a.rows, b.rows, K, BX);
     const GemmArgs<T> g{a, b, K, p.tiles_m, p.tiles_n, p.splits, p.steps_per_split, ep, static_cast<float *>(workspace)};
     const bool aligned = whole_chunks<T>(a.p, a.ld, a.extent) && whole_chunks<T>(b.p, b.ld, b.extent);
     int rc;
-    if (p.big) rc = aligned ? launch_gemm<T, AX, BX, 256, 256, 128, 64, true>(g, s) : launch_gemm<T, AX, BX, 256, 256, 128, 64, false>(g, s);
-    else rc = aligned ? launch_gemm<T, AX, BX, 128, 128, 64, 32, true>(g, s) : launch_gemm<T, AX, BX, 128, 128, 64, 32, false>(g, s);
+    auto launch = [&](auto whole) {
+        constexpr bool A = decltype(whole)::value;
+        if (p.big) return launch_gemm<T, AX, BX, 256, 256, 128, 64, A>(g, s);
+        if (p.width == 64) return launch_gemm<T, AX, BX, 128, 64, 32, 32, A>(g, s);
+        if constexpr (!BX)
+            if (p.width == 96) return launch_gemm<T, AX, BX, 128, 96, 32, 48, A>(g, s);
+        return launch_gemm<T, AX, BX, 128, 128, 64, 32, A>(g, s);
+    };
+    rc = aligned ? launch(std::true_type{}) : launch(std::false_type{});
     if (rc) return rc;
     if (p.splits > 1) {
         const int64_t outs = a.rows * ((b.rows + 3) / 4);
@@ -859,7 +741,7 @@ Slices slices_of(int64_t M, int64_t N) {
 
 extern "C" size_t detbox_linear_workspace_bytes(int dtype, int64_t M, int64_t N, int64_t K) {
     if (!dtype_ok(dtype) || M < 1 || N < 1 || K < 1) return 0;
-    return few(dtype, M, N, K) || resident(dtype, M, N, K) ? 0 : plan_bytes(plan_of(dtype, M, N, K), M, N);
+    return few(dtype, M, N, K) ? 0 : plan_bytes(plan_of(dtype, M, N, K, false), M, N);
 }
 
 extern "C" int detbox_linear_forward(int dtype, int activation, const void *x, int64_t ldx, const void *weight, int64_t ldw,
@@ -892,7 +774,7 @@ extern "C" size_t detbox_linear_backward_workspace_bytes(int dtype, int activati
     const int64_t vec = 16 / (int64_t)dtype_size(dtype), ldz = (N + vec - 1) / vec * vec;
     size_t b = align_up((size_t)slices_of(M, N).count * (size_t)N * sizeof(float), 256);
     b += align_up((size_t)M * (size_t)ldz * dtype_size(dtype), 256);
-    const size_t px = M ? plan_bytes(plan_of(dtype, M, K, N), M, K) : 0, pw = M ? plan_bytes(plan_of(dtype, N, K, M), N, K) : 0;
+    const size_t px = M ? plan_bytes(plan_of(dtype, M, K, N, true), M, K) : 0, pw = M ? plan_bytes(plan_of(dtype, N, K, M, true), N, K) : 0;
     return b + (px > pw ? px : pw);
 }
 
