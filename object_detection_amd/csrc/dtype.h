@@ -157,15 +157,7 @@ __device__ inline uint64_t group_max_u64(uint64_t v) {
     return v;
 }
 
-__device__ inline float wave_sum(float v) {
-#pragma unroll
-    for (int o = 32; o > 0; o >>= 1) v += __shfl_xor(v, o);
-    return v;
-}
-__device__ inline float wave_max(float v) {
-#pragma unroll
-    for (int o = 32; o > 0; o >>= 1) v = fmaxf(v, __shfl_xor(v, o));
-    return v;
-}
+// exp through the hardware's power of two; off by a few steps of fp32 and 2^-24 |d| relative
+__device__ inline float fast_exp(float d) { return __builtin_amdgcn_exp2f(d * 1.44269504088896340736f); }
 
 }  // namespace detbox

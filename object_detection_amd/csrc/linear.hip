@@ -24,8 +24,6 @@ typedef __attribute__((address_space(3))) s16x4 lds_s16x4;
 typedef const void __attribute__((address_space(1))) *gptr_t;
 typedef void __attribute__((address_space(3))) *lptr_t;
 
-constexpr float LOG2E = 1.44269504088896340736f;
-__device__ inline float fast_exp(float d) { return __builtin_amdgcn_exp2f(d * LOG2E); }
 __device__ inline float sigmoid_f(float z) { return __builtin_amdgcn_rcpf(1.0f + fast_exp(-z)); }
 
 // Normal distribution function by Abramowitz and Stegun, Handbook of Mathematical Functions, 7.1.26 (error below 1.5e-7 / 2);
