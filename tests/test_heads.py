@@ -625,6 +625,57 @@ def test_two_streams_at_once():
 
 
 @pytest.mark.gpu
+def test_two_threads_at_once():
+    """Calls from two host threads, each on its own stream, with autograd: the results of the calls made alone."""
+    import threading
+    g = gen(19)
+    w, b = randn(g, 300, 96), randn(g, 300)
+    xs, labels = [randn(g, 500, 96) for _ in range(2)], torch.randint(0, 300, (500,), generator=g).cuda()
+
+    def step(x):
+        x = x.detach().requires_grad_()
+        r = ops.label_log_probs(ops.linear(ops.layer_norm(x), w, b, 'gelu'), labels, 3, True)
+        return [r.log_probs.detach(), r.top_ids, torch.autograd.grad(r.log_probs.sum() + r.entropy.sum(), x)[0]]
+    want = [step(x) for x in xs]
+    torch.cuda.synchronize()
+    got, errors = [[], []], []
+
+    def work(k):
+        try:
+            with torch.cuda.stream(torch.cuda.Stream()):
+                for _ in range(20):
+                    got[k].append(step(xs[k]))
+                torch.cuda.current_stream().synchronize()
+        except Exception as e:                                          # a thread's exception would be lost otherwise
+            errors.append(e)
+    threads = [threading.Thread(target=work, args=(k,)) for k in (0, 1)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not errors
+    for k in (0, 1):
+        assert len(got[k]) == 20
+        for one in got[k]:
+            assert all(torch.equal(a, b) for a, b in zip(one, want[k]))
+
+
+@pytest.mark.gpu
+def test_no_memory_is_kept():
+    """Repeated training steps hold no more memory than one (what earlier tests left may be freed meanwhile)."""
+    g = gen(20)
+    x, w = randn(g, 3000, 200).requires_grad_(), randn(g, 90, 200).requires_grad_()
+    labels = torch.randint(0, 90, (3000,), generator=g).cuda()
+    held = []
+    for _ in range(6):
+        r = ops.label_log_probs(ops.linear(ops.layer_norm(x), w, activation='silu'), labels, 2, True)
+        torch.autograd.grad(r.log_probs.sum() + r.entropy.sum(), [x, w])
+        del r
+        held.append(torch.cuda.memory_allocated())
+    assert held[-1] <= held[1]
+
+
+@pytest.mark.gpu
 def test_rows_behind_the_last_are_left():
     """Outputs are written to their last element and not beyond: the C entry points into buffers with a guard behind."""
     L, st = _lib.lib(), torch.cuda.current_stream().cuda_stream
