@@ -624,14 +624,19 @@ bool act_ok(int act) { return act >= DETBOX_ACTIVATION_NONE && act <= DETBOX_ACT
 // as wide as the columns ask for, with the contraction in pieces where there are fewer than two tiles per CU.  Measured (bf16
 // unless it says fp32, us, large / small): 8192^3 860 / 1043, 4096^3 115 / 132, 8192 x 1024 by 8192 149 / 153, 8192 x 512 by
 // 8192 103 / 95, 65536 x 256 by 256 24 / 21, 2048^3 (64 large tiles) 59 / 31.  Width (128 / as wide as needed): 480348 x 64 by
-// 32 39 / 22, 40000 x 300 by 20 11.7 / 8.6, 120087 x 256 by 81 in fp32, where the matrix instructions count, 87 / 71.
+// 32 39 / 22, 40000 x 300 by 20 11.7 / 8.6, 120087 x 256 by 81 in fp32, where the matrix instructions count, 87 / 71; 128 / 64
+// for few tiles: 4096 x 1024 by 1024 25 / 14, 2048^3 32 / 26, 300 x 1024 by 4096 21 / 14, but 8732 x 1000 by 1208 (690 tiles)
+// 41 / 45, 512 x 4096 by 4096 (128 tiles, 64 steps) 30 / 32.
 struct Plan { bool big; int width, tiles_m, tiles_n, splits; int64_t steps_per_split; };
 Plan plan_of(int dtype, int64_t M, int64_t N, int64_t K, bool across) {
     Plan p;
     const int64_t step = 128 / (int64_t)dtype_size(dtype), steps = (K + step - 1) / step;
     p.big = ((M + 255) / 256) * ((N + 255) / 256) >= 192 && steps > 8;
     const int64_t t = p.big ? 256 : 128;
-    p.width = p.big ? 256 : N <= 64 ? 64 : N <= 96 && !across ? 96 : 128;
+    // half as wide too where whole tiles would not fill the chip: twice as many take the place of pieces and their join
+    const int64_t rows = (M + 127) / 128, whole = rows * ((N + 127) / 128), half = rows * ((N + 63) / 64);
+    const bool narrow = whole < 512 && half >= 128 && (half >= 384 || steps < 64);
+    p.width = p.big ? 256 : N <= 64 || narrow ? 64 : N <= 96 && !across ? 96 : 128;
     p.tiles_m = (int)((M + t - 1) / t);
     p.tiles_n = (int)((N + p.width - 1) / p.width);
     int64_t splits = 1;
