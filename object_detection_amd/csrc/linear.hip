@@ -6,7 +6,7 @@
 // x and W, which have that type.
 //
 // Bounds: a long contraction is bound by the matrix instructions (8192^3 bf16 1.25-1.31 PFLOP/s in all three products), a short
-// one by memory (RetinaNet's class logits, 480348 x 256 bf16 by 81, fp32 out: 88 us = 3.7 TB/s), few rows by the read of the
+// one by memory (RetinaNet's class logits, 480348 x 256 bf16 by 81, fp32 out: 88-97 us = 4.1-4.6 TB/s), few rows by the read of the
 // weight (4 x 4096 by 4096: 9 us = 3.7 TB/s).
 //
 // One tile kernel serves all three products.  Each operand lies in memory either along the contraction (x, W forward) or

@@ -125,7 +125,7 @@ __global__ __launch_bounds__(LP_BLOCK) void logprob_rows_kernel(const T *__restr
 // order, so a later equal value is not better.  The first bar is the top_k-th largest of the 64 lanes' maxima over the wave's
 // first round, which top_k logits of that round reach: on ordinary logits little more than top_k words are ever taken and
 // nothing is cut (2048 rows of 49999 fp16, five alternatives: 157 us with a buffer that is filled by the first step and cut,
-// 60 us = 3.4 TB/s so; the same rows without alternatives are bound by their read).
+// 65 us = 3.2 TB/s so).
 constexpr int BUF = 640;
 
 struct WaveBest {
