@@ -676,6 +676,49 @@ def test_no_memory_is_kept():
 
 
 @pytest.mark.gpu
+def test_accumulated_gradients_and_changed_inputs():
+    """.backward() twice adds up; an input changed in place between forward and backward is an error, not a wrong gradient."""
+    g = gen(21)
+    x, w, b = randn(g, 20, 64).requires_grad_(), randn(g, 30, 64).requires_grad_(), randn(g, 30).requires_grad_()
+    n = randn(g, 64).requires_grad_()
+    res = randn(g, 20, 30).requires_grad_()
+    labels = torch.randint(0, 30, (20,), generator=g).cuda()
+
+    def loss():
+        r = ops.label_log_probs(ops.linear(ops.layer_norm(x, n, n), w, b, 'relu', res), labels, entropy=True)
+        return r.log_probs.sum() + r.entropy.sum()
+    once = torch.autograd.grad(loss(), [x, w, b, n, res])
+    loss().backward()
+    loss().backward()
+    for leaf, v in zip((x, w, b, n, res), once):
+        assert torch.equal(leaf.grad, v + v)
+    for make in (lambda t: ops.layer_norm(t, n), lambda t: ops.linear(t, w), lambda t: ops.label_log_probs(t, labels).log_probs):
+        t = (x * 1.0)
+        y = make(t)
+        t.add_(1)
+        with pytest.raises(RuntimeError):
+            y.sum().backward()
+
+
+@pytest.mark.gpu
+def test_kernel_timing_names():
+    """The per-kernel timer knows the calls by the names the header gives."""
+    x, w = torch.randn(8, 16, device='cuda').requires_grad_(), torch.randn(4, 16, device='cuda').requires_grad_()
+    ops.profile_reset()
+    ops.profile_enable()
+    try:
+        r = ops.label_log_probs(ops.linear(ops.layer_norm(x), w), torch.zeros(8, dtype=torch.int64, device='cuda'))
+        torch.autograd.grad(r.log_probs.sum(), [x, w])
+        torch.cuda.synchronize()
+        for name in ('layer_norm', 'linear', 'label_log_probs'):
+            for way in ('forward', 'backward'):
+                assert ops.profile_read(f'{name}_{way}')[1] == 1, (name, way)
+    finally:
+        ops.profile_enable(False)
+        ops.profile_reset()
+
+
+@pytest.mark.gpu
 def test_rows_behind_the_last_are_left():
     """Outputs are written to their last element and not beyond: the C entry points into buffers with a guard behind."""
     L, st = _lib.lib(), torch.cuda.current_stream().cuda_stream
