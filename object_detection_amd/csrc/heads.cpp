@@ -116,7 +116,14 @@ struct Scratch {
     size_t bytes() const { return t.defined() ? (size_t)t.numel() : 0; }
 };
 
-Tensor shaped(const Tensor &t, at::IntArrayRef sizes) { return t.sizes() == sizes ? t : t.view(sizes); }
+// The sizes of t with the last axis replaced (none: dropped).  Outputs are allocated in their final shape: a view made inside a
+// node could not be changed in place by the caller.
+std::vector<int64_t> with_last(const Tensor &t, std::optional<int64_t> last) {
+    auto sizes = t.sizes().vec();
+    sizes.pop_back();
+    if (last) sizes.push_back(*last);
+    return sizes;
+}
 
 // The gradients of a node that has none of its own: asking for a second derivative raises, as it must.
 variable_list only_once(variable_list grads) {
@@ -147,13 +154,13 @@ struct NormResult { Tensor y, m, weight, stats; };
 NormResult norm_forward(const Tensor &x, const MaybeTensor &weight, const MaybeTensor &bias, double eps, bool keep) {
     const Tensor m = rows_of(x), w = weight ? weight->contiguous() : Tensor(), b = bias ? bias->contiguous() : Tensor();
     const int64_t rows = m.size(0), D = m.size(1);
-    Tensor y = at::empty({rows, D}, x.options()), stats;
+    Tensor y = at::empty(x.sizes(), x.options()), stats;
     if (keep) stats = at::empty({rows, 2}, x.options().dtype(at::kFloat));
     const int pdt = dtype_of(w.defined() ? w.scalar_type() : b.defined() ? b.scalar_type() : x.scalar_type());
     c10::DeviceGuard guard(x.device());
     check(api.layer_norm_forward(dtype_of(x.scalar_type()), ptr(m), stride_of(m), pdt, ptr(w), ptr(b), rows, D, (float)eps, ptr(y),
                                  fptr(stats), stream_of(x)), "detbox_layer_norm_forward");
-    return {shaped(y, x.sizes()), m, w, stats};
+    return {y, m, w, stats};
 }
 
 struct LayerNorm : torch::autograd::Function<LayerNorm> {
@@ -174,7 +181,7 @@ struct LayerNorm : torch::autograd::Function<LayerNorm> {
         {
             at::NoGradGuard none;
             const Tensor g = rows_of(grads[0]);
-            if (need & 1) gx = at::empty({rows, D}, m.options());
+            if (need & 1) gx = at::empty(ctx->saved_data["shape"].toIntVector(), m.options());
             if (need & 2) gw = at::empty({D}, m.options().dtype(param));
             if (need & 4) gb = at::empty({D}, m.options().dtype(param));
             c10::DeviceGuard guard(m.device());
@@ -182,7 +189,6 @@ struct LayerNorm : torch::autograd::Function<LayerNorm> {
             check(api.layer_norm_backward(dtype_of(m.scalar_type()), ptr(g), stride_of(g), ptr(m), stride_of(m), dtype_of(param), ptr(weight),
                                           fptr(stats), rows, D, ptr(gx), ptr(gw), ptr(gb), ws.p(), ws.bytes(), stream_of(m)),
                   "detbox_layer_norm_backward");
-            if (gx.defined()) gx = shaped(gx, ctx->saved_data["shape"].toIntVector());
         }
         return only_once({gx, gw, gb, Tensor()});
     }
@@ -211,18 +217,13 @@ LinearResult linear_forward(const Tensor &x, const Tensor &weight, const MaybeTe
     const Tensor m = rows_of(x), w = rows_of(weight), b = bias ? bias->contiguous() : Tensor(), r = residual ? rows_of(*residual) : Tensor();
     const int64_t M = m.size(0), K = m.size(1), N = w.size(0);
     const int dt = dtype_of(x.scalar_type());
-    Tensor y = at::empty({M, N}, x.options().dtype(out)), pre;
+    Tensor y = at::empty(with_last(x, N), x.options().dtype(out)), pre;
     if (keep && act) pre = at::empty({M, N}, x.options());
     c10::DeviceGuard guard(x.device());
     const Scratch ws(x, api.linear_workspace_bytes(dt, M, N, K));
     check(api.linear_forward(dt, (int)act, ptr(m), stride_of(m), ptr(w), stride_of(w), b.defined() ? dtype_of(b.scalar_type()) : 0, ptr(b), ptr(r),
                              r.defined() ? stride_of(r) : 0, M, N, K, dtype_of(out), ptr(y), ptr(pre), ws.p(), ws.bytes(), stream_of(x)),
           "detbox_linear_forward");
-    if (x.dim() != 2) {
-        auto sizes = x.sizes().vec();
-        sizes.back() = N;
-        y = y.view(sizes);
-    }
     return {y, m, w, pre};
 }
 
@@ -252,7 +253,7 @@ struct Linear : torch::autograd::Function<Linear> {
             const int64_t M = g.size(0), N = ctx->saved_data["N"].toInt(), K = shape.back(), act = ctx->saved_data["act"].toInt();
             const auto type = (at::ScalarType)ctx->saved_data["dtype"].toInt(), btype = (at::ScalarType)ctx->saved_data["bias"].toInt();
             const int dt = dtype_of(type), gdt = dtype_of(g.scalar_type());
-            if (need & 1) gx = at::empty({M, K}, g.options().dtype(type));
+            if (need & 1) gx = at::empty(shape, g.options().dtype(type));
             if (need & 2) gw = at::empty({N, K}, g.options().dtype(type));
             if (need & 4) gb = at::empty({N}, g.options().dtype(btype));
             c10::DeviceGuard guard(g.device());
@@ -260,7 +261,6 @@ struct Linear : torch::autograd::Function<Linear> {
             check(api.linear_backward(dt, (int)act, gdt, ptr(g), stride_of(g), ptr(pre), ptr(m), m.defined() ? stride_of(m) : K, ptr(w),
                                       w.defined() ? stride_of(w) : K, M, N, K, ptr(gx), ptr(gw), dtype_of(btype), ptr(gb), ws.p(), ws.bytes(),
                                       stream_of(g)), "detbox_linear_backward");
-            if (gx.defined()) gx = shaped(gx, shape);
         }
         return only_once({gx, gw, gb, need & 8 ? grads[0] : Tensor(), Tensor(), Tensor()});
     }
@@ -299,11 +299,11 @@ LogProbResult logprob_forward(const Tensor &logits, const Tensor &labels, int64_
     Tensor t = labels.scalar_type() == at::kLong ? labels : labels.to(at::kLong);
     t = t.reshape({-1}).contiguous();
     const auto f32 = logits.options().dtype(at::kFloat);
-    LogProbResult r{at::empty({rows}, f32), {}, {}, {}, m, t, {}};
-    if (entropy) r.ent = at::empty({rows}, f32);
+    LogProbResult r{at::empty(with_last(logits, std::nullopt), f32), {}, {}, {}, m, t, {}};
+    if (entropy) r.ent = at::empty_like(r.lp);
     if (top_k) {
-        r.tv = at::empty({rows, top_k}, f32);
-        r.ti = at::empty({rows, top_k}, f32.dtype(at::kLong));
+        r.tv = at::empty(with_last(logits, top_k), f32);
+        r.ti = at::empty(with_last(logits, top_k), f32.dtype(at::kLong));
     }
     if (keep) r.stats = at::empty({rows, 2}, f32);
     c10::DeviceGuard guard(logits.device());
@@ -311,17 +311,6 @@ LogProbResult logprob_forward(const Tensor &logits, const Tensor &labels, int64_
     check(api.label_log_probs_forward(dtype_of(m.scalar_type()), ptr(m), stride_of(m), static_cast<int64_t *>(ptr(t)), rows, C, (int)top_k,
                                       fptr(r.lp), fptr(r.ent), fptr(r.tv), static_cast<int64_t *>(ptr(r.ti)), fptr(r.stats), ws.p(), ws.bytes(),
                                       stream_of(logits)), "detbox_label_log_probs_forward");
-    if (logits.dim() != 2) {
-        auto lead = logits.sizes().vec();
-        lead.pop_back();
-        r.lp = r.lp.view(lead);
-        if (entropy) r.ent = r.ent.view(lead);
-        lead.push_back(top_k);
-        if (top_k) {
-            r.tv = r.tv.view(lead);
-            r.ti = r.ti.view(lead);
-        }
-    }
     return r;
 }
 
@@ -350,12 +339,11 @@ struct LogProbs : torch::autograd::Function<LogProbs> {
             at::NoGradGuard guard_grad;
             const Tensor g = grads[0].defined() ? grads[0].reshape({-1}).contiguous() : none;
             const Tensor h = grad_ent.defined() ? grad_ent.reshape({-1}).contiguous() : none;
-            gx = at::empty({m.size(0), m.size(1)}, m.options());
+            gx = at::empty(ctx->saved_data["shape"].toIntVector(), m.options());
             c10::DeviceGuard guard(m.device());
             check(api.label_log_probs_backward(dtype_of(m.scalar_type()), ptr(m), stride_of(m), static_cast<int64_t *>(ptr(t)), m.size(0),
                                                m.size(1), fptr(stats), fptr(ent), fptr(g), fptr(h), ptr(gx), stream_of(m)),
                   "detbox_label_log_probs_backward");
-            gx = shaped(gx, ctx->saved_data["shape"].toIntVector());
         }
         return only_once({gx, Tensor(), Tensor(), Tensor()});
     }

@@ -701,6 +701,32 @@ def test_accumulated_gradients_and_changed_inputs():
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize('lead', [(), (5,), (2, 3), (2, 1, 3)], ids=str)
+def test_outputs_changed_in_place(lead):
+    """Outputs of any number of axes may be changed in place, and the gradient is that of the change made out of place."""
+    g = gen(22)
+    x, w, n = randn(g, *lead, 12), randn(g, 9, 12), randn(g, 12)
+    labels = torch.randint(0, 12, lead, generator=g).cuda()
+    gate = randn(g, *lead, 12) > 0
+
+    def run(in_place):
+        leaves = [v.detach().requires_grad_() for v in (x, w, n)]
+        a = ops.layer_norm(leaves[0], leaves[2])
+        a = a.masked_fill_(gate, 0.5) if in_place else a.masked_fill(gate, 0.5)
+        b = ops.linear(a, leaves[1], activation='silu')
+        b = torch.relu_(b) if in_place else torch.relu(b)
+        r = ops.label_log_probs(leaves[0], labels, 2, True)
+        assert not r.top_log_probs.requires_grad
+        assert r.log_probs.shape == r.entropy.shape == lead and r.top_log_probs.shape == r.top_ids.shape == (*lead, 2)
+        lp = r.log_probs.mul_(3.0) if in_place else r.log_probs * 3.0
+        top = r.top_log_probs.neg_() if in_place else -r.top_log_probs
+        loss = (b * b).sum() + lp.sum() + r.entropy.sum()
+        return [b.detach(), lp.detach(), top, *torch.autograd.grad(loss, leaves)]
+    for u, v in zip(run(True), run(False)):
+        assert u.shape == v.shape and torch.equal(u, v)
+
+
+@pytest.mark.gpu
 def test_kernel_timing_names():
     """The per-kernel timer knows the calls by the names the header gives."""
     x, w = torch.randn(8, 16, device='cuda').requires_grad_(), torch.randn(4, 16, device='cuda').requires_grad_()
