@@ -146,6 +146,16 @@ bool wants_grad(std::initializer_list<const MaybeTensor *> inputs) {
     return false;
 }
 
+// Tangents are not carried through.  A call without a node would drop them without a word, which reads as a derivative of zero;
+// whether gradients are enabled or asked for does not matter to them.
+void refuse_tangents(const char *name, std::initializer_list<const MaybeTensor *> inputs) {
+    for (const auto *t : inputs)
+        if (t->has_value() && (*t)->_fw_grad(0).defined()) {
+            PyErr_SetString(PyExc_NotImplementedError, c10::str(name, " has no forward-mode derivative").c_str());
+            throw py::error_already_set();
+        }
+}
+
 Tensor value(const MaybeTensor &t) { return t.has_value() ? *t : Tensor(); }
 
 // ---- layer_norm ----------------------------------------------------------------------------------------------------------
@@ -205,6 +215,7 @@ Tensor layer_norm(const Tensor &x, const MaybeTensor &weight, const MaybeTensor 
     }
     if (weight && bias && weight->scalar_type() != bias->scalar_type()) refuse("layer_norm: weight and bias differ in type");
     const MaybeTensor xx(x);
+    refuse_tangents("layer_norm", {&xx, &weight, &bias});
     if (wants_grad({&xx, &weight, &bias})) return LayerNorm::apply(x, weight, bias, eps);
     return norm_forward(x, weight, bias, eps, false).y;
 }
@@ -286,6 +297,7 @@ Tensor linear(const Tensor &x, const Tensor &weight, const MaybeTensor &bias, in
         if (!fits) refuse("linear: residual ", residual->sizes(), " of ", residual->scalar_type(), " does not fit the output");
     }
     const MaybeTensor xx(x), ww(weight);
+    refuse_tangents("linear", {&xx, &ww, &bias, &residual});
     if (wants_grad({&xx, &ww, &bias, &residual})) return Linear::apply(x, weight, bias, residual, act, (int64_t)out);
     return linear_forward(x, weight, bias, act, residual, out, false).y;
 }
@@ -360,6 +372,7 @@ py::tuple label_log_probs(const Tensor &logits, const Tensor &labels, int64_t to
     if (top_k < 0 || top_k > std::min(most, logits.size(-1)))
         refuse("label_log_probs: top_k ", top_k, " is outside 0 .. min(", most, ", ", logits.size(-1), ")");
     const MaybeTensor x(logits);
+    refuse_tangents("label_log_probs", {&x});
     Tensor lp, ent, tv, ti;
     if (wants_grad({&x})) {
         const variable_list out = LogProbs::apply(logits, labels, top_k, entropy);

@@ -727,6 +727,29 @@ def test_outputs_changed_in_place(lead):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize('leaf', [False, True])
+def test_forward_mode_is_refused(leaf):
+    """Tangents are not carried through: a call with a dual tensor raises, also under no_grad and where no argument asks for a
+    gradient, instead of returning a value without one."""
+    import torch.autograd.forward_ad as fwAD
+    g = gen(23)
+    x, w, b, r = randn(g, 4, 8), randn(g, 6, 8), randn(g, 6), randn(g, 4, 6)
+    n, labels = randn(g, 8), torch.zeros(4, dtype=torch.int64, device='cuda')
+    calls = [(x, lambda t: ops.layer_norm(t, n, n)), (n, lambda t: ops.layer_norm(x, t, n)), (n, lambda t: ops.layer_norm(x, None, t)),
+             (x, lambda t: ops.linear(t, w, b, 'gelu', r)), (w, lambda t: ops.linear(x, t, b, 'gelu', r)), (b, lambda t: ops.linear(x, w, t)),
+             (r, lambda t: ops.linear(x, w, None, 'relu', t)), (x, lambda t: ops.label_log_probs(t, labels, 2, True))]
+    with fwAD.dual_level():
+        for v, call in calls:
+            dual = fwAD.make_dual(v.detach().requires_grad_(leaf), torch.ones_like(v))
+            with pytest.raises(NotImplementedError, match='forward-mode'):
+                call(dual)
+            with torch.no_grad(), pytest.raises(NotImplementedError, match='forward-mode'):
+                call(dual)
+        # an argument without a tangent is none: the call runs
+        assert torch.equal(ops.layer_norm(x, n, n), ops.layer_norm(x, n, n))
+
+
+@pytest.mark.gpu
 def test_kernel_timing_names():
     """The per-kernel timer knows the calls by the names the header gives."""
     x, w = torch.randn(8, 16, device='cuda').requires_grad_(), torch.randn(4, 16, device='cuda').requires_grad_()
