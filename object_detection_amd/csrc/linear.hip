@@ -3,7 +3,9 @@
 //   dz = g * act'(z),  grad_x = dz W,  grad_W = dz^T x,  grad_b = sum over rows of dz,  grad_residual = g
 // Products are summed in fp32.  What is rounded to the type of x before it is multiplied: dz (when g is wider than x or
 // there is an activation) and the z that the derivative is taken at; both are operands of the same matrix instructions as
-// x and W, which have that type.
+// x and W, which have that type.  For fp16 a dz that is rounded is first brought into that type's range by a power of two,
+// which the products take out again: a mean over many rows has gradients below fp16's smallest step, a scaled loss some beyond
+// its largest value.
 //
 // Bounds: a long contraction is bound by the matrix instructions (8192^3 bf16 1.25-1.31 PFLOP/s in all three products), a short
 // one by memory (RetinaNet's class logits, 480348 x 256 bf16 by 81, fp32 out: 88-97 us = 4.1-4.6 TB/s), few rows by the read of the
@@ -63,6 +65,7 @@ struct Epilogue {
     int act;
     void *pre; int pre_dtype;               // z, or null
     void *out; int out_dtype;
+    const float *unscale = nullptr;         // factor on the sums (in device memory), or null
 };
 
 // Four values with one (uniform) choice of the activation.
@@ -137,6 +140,7 @@ __device__ inline void store4(void *p, int dtype, int64_t i, int n, f32x4 v) {
 __device__ inline void finish4(const Epilogue &ep, int64_t row, int64_t res_row, int n, int N, f32x4 z) {
     const int left = N - n < 4 ? N - n : 4;
     if (left <= 0) return;
+    if (ep.unscale) z *= *ep.unscale;
     if (ep.bias) z += load4(ep.bias, ep.bias_dtype, n, left);
     if (ep.pre) store4(ep.pre, ep.pre_dtype, row + n, left, z);
     if (ep.act != DETBOX_ACTIVATION_NONE) z = act4(z, ep.act);
@@ -422,6 +426,10 @@ __global__ __launch_bounds__((BM / WM) * (BN / WN) * 64) void gemm_kernel(GemmAr
     float *mine = reinterpret_cast<float *>(lds) + wave * (HALF * ROW);
     const int64_t M = g.a.rows, N = g.b.rows, n = n0 + wn + (lane % LANES) * 4;
     const int left = lane >= AT_ONCE * LANES ? 0 : N - n >= 4 ? 4 : N > n ? (int)(N - n) : 0;
+    constexpr bool UNSCALE = BX && std::is_same_v<T, _Float16>;               // a product with dz
+    float unscale = 1.f;
+    if constexpr (UNSCALE)
+        if (g.ep.unscale) unscale = *g.ep.unscale;
     const f32x4 bias = g.ep.bias ? load4(g.ep.bias, g.ep.bias_dtype, n, left) : f32x4{0.f, 0.f, 0.f, 0.f};
     // A batch of U turns at a time.  The residual of a batch is on its way while the batch before it is finished (16384 x 4096
     // by 4096 bf16: a residual costs 35 us, 90 where each batch waits for its own).
@@ -471,6 +479,7 @@ __global__ __launch_bounds__((BM / WM) * (BN / WN) * 64) void gemm_kernel(GemmAr
                     store4(g.part, DETBOX_F32, (int64_t)split * M * N + at, left, z);
                     continue;
                 }
+                if constexpr (UNSCALE) z *= unscale;
                 z += bias;
                 if (g.ep.pre) store4(g.ep.pre, g.ep.pre_dtype, at, left, z);
                 if (g.ep.act != DETBOX_ACTIVATION_NONE) z = act4(z, g.ep.act);
@@ -514,16 +523,88 @@ __global__ __launch_bounds__(256) void gemm_join_kernel(const float *__restrict_
     }
 }
 
+// Largest finite |g| of a workgroup's share (0 where there is none), for the scale of an fp16 dz; the slope of no activation is
+// above 1.13, so that dz itself need not be computed for it.  A pass over g of its own: HBM bound (480348 x 81 fp32 28 us = 5.6 TB/s).
+// Dense gradients are read as one run, four packs in flight; rows with a stride LANES lanes a row.
+constexpr int PEAKS = 1024;
+__device__ inline float finite_peak(float m, float v) { return fabsf(v) < INFINITY ? fmaxf(m, fabsf(v)) : m; }
+// The largest of a workgroup's 256 values, in every thread.
+__device__ inline float block_peak(float m) {
+    __shared__ float s[4];
+    m = group_max<64>(m);
+    if ((threadIdx.x & 63) == 0) s[threadIdx.x >> 6] = m;
+    __syncthreads();
+    return fmaxf(fmaxf(s[0], s[1]), fmaxf(s[2], s[3]));
+}
+template <typename G>
+__global__ __launch_bounds__(256) void linear_peak_dense_kernel(const G *__restrict__ g, int64_t n, float *__restrict__ peaks) {
+    constexpr int VEC = VEC_OF<G>, U = 4;
+    const int64_t step = (int64_t)gridDim.x * 256 * VEC;
+    int64_t i = ((int64_t)blockIdx.x * 256 + threadIdx.x) * VEC;
+    float m = 0.f, v[U][VEC];
+    for (; i + (U - 1) * step + VEC <= n; i += U * step) {
+        detbox_u4 raw[U];
+#pragma unroll
+        for (int u = 0; u < U; ++u) raw[u] = load_raw<G>(g + i + u * step);
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            unpack<G>(v[u], raw[u]);
+#pragma unroll
+            for (int j = 0; j < VEC; ++j) m = finite_peak(m, v[u][j]);
+        }
+    }
+    for (; i < n; i += step) {
+        load_pack<G>(v[0], g + i, n - i, 0.f);
+#pragma unroll
+        for (int j = 0; j < VEC; ++j) m = finite_peak(m, v[0][j]);
+    }
+    m = block_peak(m);
+    if (threadIdx.x == 0) peaks[blockIdx.x] = m;
+}
+template <int LANES>
+__global__ __launch_bounds__(256) void linear_peak_kernel(const void *g, int gdt, int64_t ldg, int64_t M, int64_t N, float *__restrict__ peaks) {
+    constexpr int ROWS = 256 / LANES;
+    float m = 0.f;
+    for (int64_t c = ((int64_t)blockIdx.x * LANES + threadIdx.x % LANES) * 4; c < N; c += (int64_t)gridDim.x * LANES * 4) {
+        const int left = N - c >= 4 ? 4 : (int)(N - c);
+        for (int64_t row = (int64_t)blockIdx.y * ROWS + threadIdx.x / LANES; row < M; row += (int64_t)gridDim.y * ROWS) {
+            const f32x4 v = load4(g, gdt, row * ldg + c, left);
+#pragma unroll
+            for (int j = 0; j < 4; ++j) m = finite_peak(m, v[j]);
+        }
+    }
+    m = block_peak(m);
+    if (threadIdx.x == 0) peaks[blockIdx.y * gridDim.x + blockIdx.x] = m;
+}
+// The power of two that brings the largest of `count` <= PEAKS peaks to [2^14, 2^15) (at most 2^126: both it and its inverse are
+// normal numbers).  dz then stays below 2^15.2, inside fp16, and what a small dz loses is at most half of fp16's smallest step,
+// 2^-39 of the largest gradient.  For all 256 threads of a workgroup.
+__device__ inline int scale_exponent(const float *peaks, int count) {
+    float m = 0.f;
+    for (int i = threadIdx.x; i < count; i += 256) m = fmaxf(m, peaks[i]);
+    m = block_peak(m);
+    if (m == 0.f) return 0;
+    const int e = 14 - ((int)(__float_as_uint(m) >> 23) - 127);
+    return e < 126 ? e : 126;
+}
+
 // dz = g * act'(pre) in the type of x with rows of ldz elements (zeros behind N), and partial column sums of the unrounded dz
-// per row slice.  LANES lanes share a row, four columns each; HBM bound (16384 x 4096 bf16 with gelu: 96 us = 4.2 TB/s).
+// per row slice.  With peaks, dz is stored times their power of two, the inverse of which goes to *unscale.  LANES lanes share a row, four columns each; HBM bound (16384 x 4096 bf16 with gelu: 96 us = 4.2 TB/s).
 template <typename T, int LANES>
 __global__ __launch_bounds__(256) void linear_slope_kernel(const void *g, int gdt, int64_t ldg, const T *__restrict__ pre, int act,
                                                            int64_t M, int64_t N, int64_t ldz, int64_t rows_per_slice,
-                                                           T *__restrict__ dz, float *__restrict__ part) {
+                                                           T *__restrict__ dz, float *__restrict__ part,
+                                                           const float *__restrict__ peaks, int n_peaks, float *__restrict__ unscale) {
     constexpr int DT = sizeof(T) == 4 ? DETBOX_F32 : std::is_same_v<T, __bf16> ? DETBOX_BF16 : DETBOX_F16, ROWS = 256 / LANES;
     const int lane = threadIdx.x % LANES;
     const int64_t c = ((int64_t)blockIdx.x * LANES + lane) * 4;
     const int left = N - c >= 4 ? 4 : N - c > 0 ? (int)(N - c) : 0, room = ldz - c < 4 ? (int)(ldz - c) : 4;
+    int up = 0;                             // ldexp, not a product: the products cost 45 us at 16384 x 4096 (98 against 143)
+    if constexpr (std::is_same_v<T, _Float16>)
+        if (peaks) {
+            up = scale_exponent(peaks, n_peaks);
+            if (blockIdx.x == 0 && blockIdx.y == 0 && threadIdx.x == 0) *unscale = __uint_as_float((uint32_t)(127 - up) << 23);
+        }
     f32x4 a = {0.f, 0.f, 0.f, 0.f};
     const int64_t lo = blockIdx.y * rows_per_slice, hi = lo + rows_per_slice < M ? lo + rows_per_slice : M;
     if (c < ldz) {
@@ -533,7 +614,11 @@ __global__ __launch_bounds__(256) void linear_slope_kernel(const void *g, int gd
         for (int64_t row = row0; row < hi; row += ROWS, at_g += by_g, at_p += by_p, at_z += by_z) {
             f32x4 v = load4(g, gdt, at_g, left);
             if (pre) v *= slope4(load4(pre, DT, at_p, left), act);                // v is 0 behind N
-            if (dz) store4(dz, DT, at_z, room, v);
+            if (dz) {
+                f32x4 d = v;
+                if constexpr (std::is_same_v<T, _Float16>) d = f32x4{ldexpf(v[0], up), ldexpf(v[1], up), ldexpf(v[2], up), ldexpf(v[3], up)};
+                store4(dz, DT, at_z, room, d);
+            }
             a += v;
         }
     }
@@ -786,6 +871,7 @@ extern "C" size_t detbox_linear_backward_workspace_bytes(int dtype, int activati
     const int64_t vec = 16 / (int64_t)dtype_size(dtype), ldz = (N + vec - 1) / vec * vec;
     size_t b = align_up((size_t)slices_of(M, N).count * (size_t)N * sizeof(float), 256);
     b += align_up((size_t)M * (size_t)ldz * dtype_size(dtype), 256);
+    if (dtype == DETBOX_F16) b += align_up((PEAKS + 1) * sizeof(float), 256);
     const size_t px = M ? plan_bytes(plan_of(dtype, M, K, N, true), M, K) : 0, pw = M ? plan_bytes(plan_of(dtype, N, K, M, true), N, K) : 0;
     return b + (px > pw ? px : pw);
 }
@@ -813,16 +899,34 @@ extern "C" int detbox_linear_backward(int dtype, int activation, int grad_dtype,
         using T = decltype(t);
         const int64_t padded = (N + VEC_OF<T> - 1) / VEC_OF<T> * VEC_OF<T>;
         T *dz = ws.take<T>((size_t)M * padded);
+        float *peaks = dtype == DETBOX_F16 ? ws.take<float>(PEAKS + 1) : nullptr, *unscale = nullptr;
         void *pieces = ws.take<char>(0);
         const bool slope = activation != DETBOX_ACTIVATION_NONE;
         // dz is written out where it is not g itself, or where g's rows start off 16 bytes
         const bool convert = slope || grad_dtype != dtype || !whole_chunks<T>(grad_y, ldg, N);
+        // an fp16 dz that has other digits than g (which has its type, and relu keeps or drops it) is scaled into range
+        const bool scaled = M && dtype == DETBOX_F16 && (grad_x || grad_weight) &&
+                            (grad_dtype != dtype || (slope && activation != DETBOX_ACTIVATION_RELU));
+        if (scaled) unscale = peaks + PEAKS;
         if (M && (convert || grad_bias)) {
             auto launch = [&](auto lanes) {
                 constexpr int LANES = decltype(lanes)::value;
+                int n_peaks = 0;
+                if (scaled && (ldg == N || M == 1)) {
+                    const int64_t n = M * N, blocks = (n + 1023) / 1024;
+                    n_peaks = blocks < PEAKS ? (int)blocks : PEAKS;
+                    const dim3 grid((unsigned)n_peaks), block(256);
+                    if (grad_dtype == DETBOX_F32) linear_peak_dense_kernel<<<grid, block, 0, s>>>(static_cast<const float *>(grad_y), n, peaks);
+                    else linear_peak_dense_kernel<<<grid, block, 0, s>>>(static_cast<const _Float16 *>(grad_y), n, peaks);
+                } else if (scaled) {
+                    const int64_t by_rows = (M + 256 / LANES - 1) / (256 / LANES), by_columns = (N + LANES * 4 - 1) / (LANES * 4);
+                    const int64_t y = by_rows < PEAKS ? by_rows : PEAKS, x = by_columns < PEAKS / y ? by_columns : PEAKS / y;
+                    n_peaks = (int)(x * y);
+                    linear_peak_kernel<LANES><<<dim3((unsigned)x, (unsigned)y), dim3(256), 0, s>>>(grad_y, grad_dtype, ldg, M, N, peaks);
+                }
                 linear_slope_kernel<T, LANES><<<dim3((unsigned)((padded + LANES * 4 - 1) / (LANES * 4)), sl.count), dim3(256), 0, s>>>(
                     grad_y, grad_dtype, ldg, slope ? static_cast<const T *>(pre_activation) : nullptr, activation, M, N, padded, sl.rows,
-                    convert ? dz : nullptr, grad_bias ? part : nullptr);
+                    convert ? dz : nullptr, grad_bias ? part : nullptr, scaled ? peaks : nullptr, n_peaks, unscale);
             };
             if (padded <= 32) launch(std::integral_constant<int, 8>{});
             else if (padded <= 128) launch(std::integral_constant<int, 32>{});
@@ -830,7 +934,7 @@ extern "C" int detbox_linear_backward(int dtype, int activation, int grad_dtype,
         }
         const T *z = convert ? dz : static_cast<const T *>(grad_y);
         const int64_t ldz = convert ? padded : ldg, z_end = convert ? padded : N;
-        Epilogue ep{nullptr, 0, nullptr, 0, DETBOX_ACTIVATION_NONE, nullptr, 0, grad_x, dtype};
+        Epilogue ep{nullptr, 0, nullptr, 0, DETBOX_ACTIVATION_NONE, nullptr, 0, grad_x, dtype, unscale};
         // the zeros behind N let the contraction over N run in whole chunks; the weight's rows end there
         if (grad_x && M) rc = gemm<T, false, true>({z, ldz, M, z_end}, {static_cast<const T *>(weight), ldw, K, K}, N, dtype, ep, pieces, s);
         ep.out = grad_weight;

@@ -558,7 +558,8 @@ def linear(x: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Tensor] =
     activation one of ACTIVATIONS, residual [..., N] of the output's type, which is that of x or, with
     out_dtype=torch.float32, the fp32 sum itself (the logits select_decode and focal_loss_sum take).  Differentiable in x,
     weight, bias and residual; products are summed in fp32, the gradient at the activation's input is rounded to the type
-    of x before it is multiplied."""
+    of x before it is multiplied (float16: scaled into range by a power of two first, so that gradients far below or above
+    that type's range count too)."""
     act = ACTIVATIONS.get(activation)
     if act is None:
         raise ValueError(f'linear: unknown activation {activation!r}')

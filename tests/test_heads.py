@@ -297,6 +297,74 @@ def test_linear_whole_values(dtype):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize('M,N,K', [(3, 20, 40), (70, 81, 256), (700, 203, 96), (5000, 81, 64), (3600, 3704, 3656)])
+@pytest.mark.parametrize('act,out', [('none', torch.float32), ('gelu', torch.float32), ('relu', torch.float32), ('silu', torch.float16),
+                                     ('sigmoid', torch.float32)])
+def test_half_gradients_keep_their_range(M, N, K, act, out):
+    """fp16 operands with gradients far below and far above fp16's range, up to 2^30 apart in one call: dz is brought into range by a power of two
+    before it is rounded, so that beside the half step of every element only 2^-39 of the largest gradient is lost (the smallest
+    step of fp16 is 2^-24, the largest gradient lies at 2^14 or above, half a step is 2^-25)."""
+    g = torch.Generator(device='cuda').manual_seed(M + N + K)
+
+    def rand(*shape, scale=1.0, dtype=torch.float32):
+        return (torch.randn(*shape, generator=g, device='cuda') * scale).to(dtype)
+    x, w = rand(M, K, dtype=torch.float16), rand(N, K, scale=K ** -0.5, dtype=torch.float16)
+    b = rand(N)
+    wide = torch.exp2(torch.randint(-30, 1, (M, N), generator=g, device='cuda').float())
+    grads = {'mean': rand(M, N, scale=2.0 ** -26), 'wide': rand(M, N) * wide, 'zero': torch.zeros(M, N, device='cuda')}
+    if out == torch.float32:
+        grads.update(large=rand(M, N, scale=2.0 ** 20), small=rand(M, N, scale=2.0 ** -100), wide_large=rand(M, N, scale=2.0 ** 18) * wide,
+                     strided=rand(M, N + 5, scale=2.0 ** -26)[:, 3:N + 3])
+    else:
+        grads = {k: (v * 2.0 ** 14 if k == 'mean' else v).half() for k, v in grads.items()}
+    bb = b.clone().requires_grad_()
+    # gradients below fp16's range leave it again only through an output: x and the weight carry them up by powers of two
+    for name, gr in grads.items():
+        up = 2.0 ** {'large': -14, 'wide_large': -14, **({'mean': 10, 'small': 13, 'strided': 10} if act == 'none' else {})}.get(name, 0)
+        xs, ws = [(v * up).half() for v in (x.float(), w.float())]
+        leaves = [xs.requires_grad_(), ws.requires_grad_(), bb]
+        y = ops.linear(leaves[0], leaves[1], bb, act, None, out)
+        gx, gw, gb = torch.autograd.grad(y, leaves, gr)
+        xd, wd, gd = xs.detach().double(), ws.detach().double(), gr.double()
+        z = xd @ wd.t() + b.double()
+        ez = (K + 4) * E * (xd.abs() @ wd.abs().t()) + 2 * E * (z.abs() + b.double().abs())
+        _, slope, _, bend = act_def(z, act)
+        dz = gd * slope
+        es = 0.0
+        if act == 'relu':
+            es = (z.abs() <= ez + TINY[torch.float16]).double()
+        elif act != 'none':
+            es = 24 * E * (1 + z.abs()) + bend * (ez + U[torch.float16] * (z.abs() + ez) + TINY[torch.float16])
+        edz = gd.abs() * es + E * dz.abs()
+        rounded = edz + U[torch.float16] * (dz.abs() + edz) + 2.0 ** -39 * gd.abs().max()
+        for got, want, tol, what in ((gx, dz @ wd, rounded @ wd.abs() + (N + 4) * E * ((dz.abs() + rounded) @ wd.abs()), 'x'),
+                                     (gw, dz.t() @ xd, rounded.t() @ xd.abs() + (M + 4) * E * ((dz.abs() + rounded).t() @ xd.abs()), 'w'),
+                                     (gb, dz.sum(0), edz.sum(0) + (M + 4) * E * (dz.abs() + edz).sum(0), 'b')):
+            # 2^-126: fp32 sums of the smallest gradients may be flushed
+            close(got, want, tol + U[got.dtype] * (want.abs() + tol) + TINY[got.dtype] + 2.0 ** -126, f'{name} {what}')
+        if name in ('mean', 'large') and act == 'none':
+            assert gx.any() and gw.any() and torch.isfinite(gx).all()
+
+
+@pytest.mark.gpu
+def test_half_gradients_beyond_numbers():
+    """Infinities and NaN among the gradients stay in their row and column and leave the scale of the others alone."""
+    g = gen(24)
+    x, w = randn(g, 90, 64, dtype=torch.float16).requires_grad_(), randn(g, 50, 64, dtype=torch.float16).requires_grad_()
+    gr = randn(g, 90, 50, scale=2.0 ** -10)
+    clean = torch.autograd.grad(ops.linear(x, w, out_dtype=torch.float32), [x, w], gr.index_fill(0, torch.tensor([7, 30], device='cuda'), 0.0))
+    for bad in (math.inf, -math.inf, math.nan):
+        gr2 = gr.clone()
+        gr2[7], gr2[30] = 0.0, 0.0
+        gr2[7, 3], gr2[30, 3] = bad, bad
+        gx, gw = torch.autograd.grad(ops.linear(x, w, out_dtype=torch.float32), [x, w], gr2)
+        keep_m, keep_n = torch.ones(90, dtype=torch.bool), torch.ones(50, dtype=torch.bool)
+        keep_m[[7, 30]], keep_n[3] = False, False
+        assert not torch.isfinite(gx[~keep_m]).any() and torch.equal(gx[keep_m][:, :], clean[0][keep_m])
+        assert not torch.isfinite(gw[3]).any() and torch.equal(gw[keep_n], clean[1][keep_n])
+
+
+@pytest.mark.gpu
 def test_linear_no_rows():
     x, w = torch.zeros(0, 6, device='cuda', requires_grad=True), torch.ones(4, 6, device='cuda', requires_grad=True)
     b = torch.ones(4, device='cuda', requires_grad=True)
