@@ -193,7 +193,7 @@ int detbox_layer_norm_backward(int dtype, const void *grad_y, int64_t ldg, const
  * grad_weight [N,K], grad_bias [N] is not NULL; the residual's gradient is grad_y itself.  pre_activation may be NULL
  * with DETBOX_ACTIVATION_NONE, weight where grad_x is, x where grad_weight is.
  * The gradient at x W^T + bias is rounded to `dtype` before it is multiplied, and the slope is taken at pre_activation, which
- * has that type too.  For DETBOX_F16 the gradient is brought into range by a power of two first and the products are scaled
+ * has that type too (DETBOX_F16: values in (0, 2^-24) are kept as 2^-24).  For DETBOX_F16 the gradient is brought into range by a power of two first and the products are scaled
  * back: what is lost of a small element is at most 2^-39 of the largest |grad_y|, and none overflows. */
 size_t detbox_linear_workspace_bytes(int dtype, int64_t M, int64_t N, int64_t K);
 int detbox_linear_forward(int dtype, int activation, const void *x, int64_t ldx, const void *weight, int64_t ldw,

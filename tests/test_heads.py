@@ -365,6 +365,30 @@ def test_half_gradients_beyond_numbers():
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize('M,N,K', [(2, 20, 8), (2, 20, 2048), (150, 40, 64), (150, 40, 2048), (40, 2000, 4096), (3600, 3700, 640)])
+def test_half_relu_keeps_the_sign_of_small_sums(M, N, K):
+    """Sums of 2^-28 and -2^-28, below half of fp16's smallest step: the slope of relu is 1 and 0 there, not 0 twice.  All of
+    it in powers of two, so that the gradients are exact."""
+    x, w = torch.zeros(M, K, dtype=torch.float16, device='cuda'), torch.zeros(N, K, dtype=torch.float16, device='cuda')
+    x[:, K - 1] = 2.0 ** -14
+    w[:, K - 1] = 2.0 ** -14
+    w[1::2] *= -1
+    gr = torch.zeros(M, N, dtype=torch.float16, device='cuda')
+    gr[:2, :4] = 1.0
+    for b in (None, torch.zeros(N, device='cuda')):
+        for out in (None, torch.float32):
+            leaves = [x.requires_grad_(), w.requires_grad_()]
+            y = ops.linear(*leaves, b, 'relu', None, out)
+            gx, gw = torch.autograd.grad(y, leaves, gr.to(out or torch.float16))
+            want_x, want_w = torch.zeros_like(x), torch.zeros_like(w)
+            want_x[:2, K - 1] = 2 * 2.0 ** -14
+            want_w[0:4:2, K - 1] = 2 * 2.0 ** -14
+            assert torch.equal(gx, want_x) and torch.equal(gw, want_w)
+            if out:
+                assert torch.equal(y.detach(), torch.where(torch.arange(N, device='cuda') % 2 == 0, 2.0 ** -28, 0.0).expand(M, N))
+
+
+@pytest.mark.gpu
 def test_linear_no_rows():
     x, w = torch.zeros(0, 6, device='cuda', requires_grad=True), torch.ones(4, 6, device='cuda', requires_grad=True)
     b = torch.ones(4, device='cuda', requires_grad=True)
