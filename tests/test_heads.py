@@ -981,6 +981,31 @@ def test_offsets_beyond_32_bits():
 
 
 @pytest.mark.gpu
+def test_columns_beyond_one_grid():
+    """More columns than one grid of the column sums has threads for (2^27 sums of 32 threads each): with one row the sums are
+    the row's own products, which are exact."""
+    t = torch.bfloat16
+    n = (1 << 26) + 37
+    x = torch.zeros(1, n, dtype=t, device='cuda')
+    x[0, ::2], x[0, n - 1] = 1.0, -1.0
+    gr = (torch.arange(n, device='cuda') % 251).to(t)[None]
+    w, b = torch.ones(n, dtype=t, device='cuda').requires_grad_(), torch.zeros(n, dtype=t, device='cuda').requires_grad_()
+    y = ops.layer_norm(x, w, b)
+    gw, gb = torch.autograd.grad(y, [w, b], gr)
+    assert torch.equal(gb, gr[0])
+    # the ends of the axis, each within one rounding of gradient times output (weight 1, bias 0: the output is h, rounded)
+    for part in (slice(0, 4096), slice(n // 2, n // 2 + 4096), slice(n - 4096, n)):
+        want = gr[0, part].double() * y.detach()[0, part].double()
+        assert ((gw[part].double() - want).abs() <= 2.0 ** -7 * 1.01 * want.abs()).all()
+    del x, gr, w, b, y, gw, gb
+    n = (1 << 27) + 37
+    w, x = torch.ones(n, 1, dtype=t, device='cuda'), torch.ones(1, 1, dtype=t, device='cuda')
+    b = torch.zeros(n, dtype=t, device='cuda').requires_grad_()
+    gr = (torch.arange(n, device='cuda') % 251).to(t)[None]
+    assert torch.equal(torch.autograd.grad(ops.linear(x, w, b), b, gr)[0], gr[0])
+
+
+@pytest.mark.gpu
 def test_library_errors_are_the_packages():
     """A limit of the library arrives as DetboxError."""
     with pytest.raises(_lib.DetboxError, match='DETBOX_LINEAR_MAX_TILES'):
