@@ -7,7 +7,7 @@ network part (forward, backbone, heads) alone; `Predictor` of this package repla
 """
 from __future__ import annotations
 
-from .models import MODELS
+from .models import MODELS, _BoxOps
 
 
 def bind_boxops(model, name: str, **ctor):
@@ -16,12 +16,15 @@ def bind_boxops(model, name: str, **ctor):
     class count -- `f_k_list` (feature-map sizes) for RetinaNet and FCOS, whose tables the reference builds from
     the first forward (src/models/retinanet.py:116-117).
     The reference stores `nc = num_classes + 1` for the soft-max heads (src/models/ssd300.py:57) and
-    `nc = num_classes` for YOLOv3; the box-ops constructors take num_classes."""
+    `nc = num_classes` for YOLOv3; the box-ops constructors take num_classes.
+    A model's own `head_logits` (a method, a submodule) stays what it is; `model.boxops.head_logits` is there in any case."""
     num_classes = model.nc if name == 'yolov3' else model.nc - 1
     impl = MODELS[name](num_classes, **ctor)
     model.boxops = impl
     model.loss = impl.loss
     model.pre_predict = impl.pre_predict
     model.detect = impl.detect
-    model.head_logits = impl.head_logits
+    own = getattr(model, 'head_logits', None)
+    if own is None or isinstance(getattr(own, '__self__', None), _BoxOps):     # none, or that of an earlier binding
+        model.head_logits = impl.head_logits
     return model

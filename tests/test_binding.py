@@ -57,6 +57,31 @@ def test_integration_snippet_binds_the_reference_seams():
     assert list(inspect.signature(D.Predictor.__init__).parameters) == ['self', 'iou_thresh', 'classes', 'out_dir']
 
 
+def test_binding_leaves_a_models_own_head_logits_alone():
+    """No GPU needed: a submodule or a method of that name belongs to the network part; without one the box-ops' is bound, and a
+    second binding replaces the first's."""
+    import object_detection_amd as D
+
+    class WithModule(torch.nn.Module):
+        def __init__(self):
+            super().__init__()
+            self.nc = 21
+            self.head_logits = torch.nn.Linear(4, 21)
+
+    class WithMethod(StandInModel):
+        def head_logits(self, x):
+            return 'the network\'s'
+    m = WithModule()
+    layer = m.head_logits
+    assert D.bind_boxops(m, 'ssd300').head_logits is layer and len(list(m.parameters())) == 2
+    assert m.boxops.head_logits.__self__ is m.boxops
+    assert D.bind_boxops(WithMethod(21), 'ssd300').head_logits(None) == "the network's"
+    plain = StandInModel(21)
+    for _ in range(2):
+        D.bind_boxops(plain, 'ssd300')
+        assert plain.head_logits.__self__ is plain.boxops
+
+
 def test_candidate_lists_are_plain_lists_with_a_link():
     """No GPU needed: the lists pre_predict returns behave as lists; recall() only follows untouched ones."""
     from object_detection_amd import predictor as P
