@@ -10,6 +10,7 @@ have given wrong results on this hardware now and then.
 """
 import glob
 import os
+import shutil
 import subprocess
 import sys
 from concurrent.futures import ThreadPoolExecutor
@@ -66,11 +67,17 @@ def build_heads(verbose=False):
     return HEADS_OUT
 
 
-def build(force=False, verbose=False):
-    if force or heads_need_build():
-        build_heads(verbose)
-    if not force and not needs_build():
-        return OUT
+def heads_missing():
+    """What building the autograd nodes lacks, or None."""
+    try:
+        import torch  # noqa: F401
+    except ImportError:
+        return 'PyTorch is not importable'
+    cxx = os.environ.get('CXX', 'g++')
+    return None if shutil.which(cxx) else f'no host compiler {cxx}'
+
+
+def build_library(verbose=False):
     hipcc = os.environ.get('HIPCC', '/opt/rocm/bin/hipcc')
     os.makedirs(OBJ, exist_ok=True)
 
@@ -85,6 +92,22 @@ def build(force=False, verbose=False):
     with ThreadPoolExecutor(max_workers=min(8, len(sources()))) as ex:
         objs = list(ex.map(compile_one, sources()))
     subprocess.check_call([hipcc, '--offload-arch=gfx950', '-shared', '-fPIC', '-o', OUT] + objs)
+    return OUT
+
+
+def build(force=False, verbose=False):
+    """The library first: it needs hipcc only, and is all that a user of the C ABI needs.  The autograd nodes follow where PyTorch and a
+    host compiler are there."""
+    if force or needs_build():
+        build_library(verbose)
+    if force or heads_need_build():
+        missing = heads_missing()
+        if not missing:
+            build_heads(verbose)
+        else:
+            if os.path.exists(HEADS_OUT):                           # of other sources: not left to be loaded
+                os.unlink(HEADS_OUT)
+            print(f'{os.path.basename(HEADS_OUT)} (the class-head operators for PyTorch) is not built: {missing}', file=sys.stderr)
     return OUT
 
 

@@ -95,3 +95,39 @@ def test_release_workspaces_empties_the_cache():
     ops._workspaces[(1, 'probe', 0)] = torch.empty(512, dtype=torch.uint8)
     assert ops.release_workspaces('cuda:1') == 512 and (0, 'probe', 0) in ops._workspaces
     assert ops.release_workspaces() == 1024 and not ops._workspaces
+
+
+@pytest.mark.parametrize('lacking', ['pytorch', 'compiler', 'headers', None])
+def test_build_makes_the_c_library_whatever_the_autograd_nodes_lack(monkeypatch, tmp_path, capsys, lacking):
+    """A user of the C ABI needs hipcc only: the library is compiled and linked first, and without PyTorch or a host compiler the nodes
+    are left out with a word (and no binary of other sources stays).  Nothing is compiled here: the commands are recorded."""
+    import subprocess
+    import sys
+
+    from object_detection_amd import build
+    ran = []
+
+    def record(cmd, *a, **k):
+        ran.append(list(cmd))
+        if lacking == 'headers' and build.HEADS_SRC in cmd:
+            raise subprocess.CalledProcessError(1, cmd)
+    stale = tmp_path / '_heads.so'
+    stale.write_bytes(b'')
+    os.utime(stale, (1, 1))
+    monkeypatch.setattr(build, 'HEADS_OUT', str(stale))
+    monkeypatch.setattr(build, 'OBJ', str(tmp_path))
+    monkeypatch.setattr(subprocess, 'check_call', record)
+    if lacking == 'pytorch':
+        monkeypatch.setitem(sys.modules, 'torch', None)
+    if lacking == 'compiler':
+        monkeypatch.setenv('CXX', str(tmp_path / 'no_such_compiler'))
+    if lacking == 'headers':
+        with pytest.raises(subprocess.CalledProcessError):              # a nodes' build that fails is an error
+            build.build(force=True)
+    else:
+        assert build.build(force=True) == build.OUT
+    library = [c for c in ran if build.HEADS_SRC not in c]
+    assert len(library) == len(build.sources()) + 1 and build.OUT in library[-1]
+    assert ran[:len(library)] == library and len(ran) - len(library) == (lacking in ('headers', None))
+    said = 'is not built' in capsys.readouterr().err
+    assert said == (lacking in ('pytorch', 'compiler')) == (not stale.exists())
