@@ -22,6 +22,11 @@ __device__ inline uint64_t rank_word(float v, uint32_t i) {
     return ((uint64_t)k << 32) | (uint32_t)~i;
 }
 
+// Distances from the largest logit where they are multiplied by their exponential, or by what meets it: no further than this, at
+// which (and from -104 on) the exponential is 0 in fp32, so that the product is 0 too and not -inf * 0.  A sum of 2^31 terms or a
+// gradient of 2^100 times it stays finite.
+constexpr float FAR = -1e4f;
+
 // A row's results from its largest logit (0 where it is -inf) and its sums.
 struct RowSums { float ref, sum, dot; };        // sum of e = exp(x - ref), sum of e * (x - ref)
 __device__ inline bool no_distribution(float m, float sum) { return m == -INFINITY && sum == 0.f; }
@@ -32,7 +37,7 @@ __device__ inline void merge_sums(float &m, float &s, float &t, float m2, float 
     const float ref = n == -INFINITY ? 0.f : n;
     const float d1 = m - ref, d2 = m2 - ref;                       // -inf for a side without a finite logit: its sums are 0
     const float e1 = fast_exp(d1), e2 = fast_exp(d2);
-    t = e1 * fmaf(s, fmaxf(d1, -1e30f), t) + e2 * fmaf(s2, fmaxf(d2, -1e30f), t2);
+    t = e1 * fmaf(s, fmaxf(d1, FAR), t) + e2 * fmaf(s2, fmaxf(d2, FAR), t2);
     s = s * e1 + s2 * e2;
     m = n;
 }
@@ -93,7 +98,7 @@ __global__ __launch_bounds__(LP_BLOCK) void logprob_rows_kernel(const T *__restr
             for (int i = 0; i < VEC; ++i) {
                 const float d = v[q][i] - ref, e = fast_exp(d);
                 s += e;
-                if (o.entropy) t = fmaf(e, fmaxf(d, -1e30f), t);
+                if (o.entropy) t = fmaf(e, fmaxf(d, FAR), t);
             }
         s = group_sum<G>(s);
         if (o.entropy) t = group_sum<G>(t);
@@ -306,7 +311,7 @@ __global__ __launch_bounds__(LP_BLOCK) void logprob_long_kernel(const T *__restr
             for (int i = 1; i < VEC; ++i) top = fmaxf(top, v[i]);
             if (top > m) {
                 const float d = m - top, e = fast_exp(d);                  // m == -inf: e = 0 and both sums are 0
-                if (ENT) t = e * fmaf(s, fmaxf(d, -1e30f), t);
+                if (ENT) t = e * fmaf(s, fmaxf(d, FAR), t);
                 s *= e;
                 m = top;
             }
@@ -315,7 +320,7 @@ __global__ __launch_bounds__(LP_BLOCK) void logprob_long_kernel(const T *__restr
             for (int i = 0; i < VEC; ++i) {
                 const float d = v[i] - ref, e = fast_exp(d);
                 s += e;
-                if (ENT) t = fmaf(e, fmaxf(d, -1e30f), t);
+                if (ENT) t = fmaf(e, fmaxf(d, FAR), t);
             }
             return top;
         };
@@ -485,7 +490,7 @@ __device__ inline void grad_pack(float (&v)[VEC], const RowGrad &r, int64_t c) {
 #pragma unroll
     for (int i = 0; i < VEC; ++i) {
         const float d = v[i] - r.ref, p = fast_exp(d) * r.inv;
-        v[i] = -p * fmaf(r.h, fmaxf(d, -1e30f), r.a);
+        v[i] = -p * fmaf(r.h, fmaxf(d, FAR), r.a);
     }
     const int64_t at = r.label - c;
     if (at >= 0 && at < VEC) {

@@ -566,6 +566,24 @@ def test_label_log_probs_no_rows():
     assert torch.autograd.grad(r.log_probs.sum() + r.entropy.sum(), x)[0].shape == (0, 9)
 
 
+@pytest.mark.gpu
+@pytest.mark.parametrize('dtype', TYPES, ids=str)
+@pytest.mark.parametrize('C', [5, 300, 5000])
+def test_entropy_gradient_of_classes_that_cannot_be(dtype, C):
+    """A large gradient of the entropy leaves classes of -inf and of the type's lowest value at 0: their probability is."""
+    g = gen(25)
+    x = randn(g, 3, C, dtype=dtype)
+    x[:, 1], x[:, C - 1] = -math.inf, torch.finfo(dtype).min
+    x.requires_grad_()
+    r = ops.label_log_probs(x, torch.full((3,), -1, device='cuda'), entropy=True)
+    small = torch.autograd.grad(r.entropy, x, torch.full((3,), 2.0 ** -10, device='cuda'), retain_graph=True)[0]
+    for h in (2.0 ** 30, -2.0 ** 40):
+        gx = torch.autograd.grad(r.entropy, x, torch.full((3,), h, device='cuda'), retain_graph=True)[0]
+        assert not gx[:, [1, C - 1]].any() and not torch.isnan(gx).any()
+        if dtype is torch.float32:                                      # powers of two: the same digits
+            assert torch.equal(gx, small * (h * 2.0 ** 10))
+
+
 # ------------------------------------------------------------------ all of them
 
 @pytest.mark.gpu
