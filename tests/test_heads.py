@@ -658,6 +658,28 @@ def test_head_logits_train_and_detect():
 
 @pytest.mark.gpu
 @pytest.mark.parametrize('dtype', TYPES, ids=str)
+def test_head_logits_train_on_a_mean_over_many_anchors(dtype):
+    """The mean of the log probabilities over 120000 anchors of 81 classes: most of its gradients at the logits are near 1e-7.  Those
+    of the features and the embeddings against the definition in 64 bits, from the same gradients at the logits: dz is off by half
+    a step of the features' type (none in fp32) and, in fp16, by 2^-39 of the largest; then sums of n fp32 terms, rounded once."""
+    g = torch.Generator(device='cuda').manual_seed(26)
+    m = D.RetinaNet(80, [8, 4, 2, 1, 1])
+    feats = torch.randn(4, 30000, 64, generator=g, device='cuda').to(dtype).requires_grad_()
+    emb = (torch.randn(m.nc, 64, generator=g, device='cuda') / 8).to(dtype).requires_grad_()
+    labels = torch.randint(0, m.nc, (4, 30000), generator=g, device='cuda')
+    logits = m.head_logits(feats, emb)
+    assert logits.shape == (4, 30000, 81) and logits.dtype == torch.float32
+    top, gf, ge = torch.autograd.grad(ops.label_log_probs(logits, labels).log_probs.mean(), [logits, feats, emb])
+    dz, fd, ed = top.double().reshape(-1, 81), feats.detach().double().reshape(-1, 64), emb.detach().double()
+    off = (U[dtype] * dz.abs() + 2.0 ** -39 * dz.abs().max() if dtype != torch.float32 else torch.zeros_like(dz))
+    for got, want, tol in ((gf.reshape(-1, 64), dz @ ed, off @ ed.abs() + 85 * E * ((dz.abs() + off) @ ed.abs())),
+                           (ge, dz.t() @ fd, off.t() @ fd.abs() + 120004 * E * ((dz.abs() + off).t() @ fd.abs()))):
+        close(got, want, tol + U[dtype] * (want.abs() + tol) + TINY[dtype])
+    assert float((ge.double() - dz.t() @ fd).norm()) <= 4 * U[dtype] * float((dz.t() @ fd).norm()) + 120004 * E * float((dz.abs().t() @ fd.abs()).norm())
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize('dtype', TYPES, ids=str)
 def test_streams_and_graphs(dtype):
     """On a stream of its own, and captured (forward and backward) into graphs that are replayed with new inputs and eager
     calls between: every replay gives the eager result's bits.  Two graphs captured one after the other share nothing."""
