@@ -136,10 +136,10 @@ __device__ inline void store4(void *p, int dtype, int64_t i, int n, f32x4 v) {
 
 // z as it is kept for the slope.  fp16 holds nothing between 0 and 2^-24: what lies there is kept as the latter, since relu's
 // slope is 1 at any z above 0 and 0 at 0 itself (the other slopes are the same at both to 2^-24).
-__device__ inline f32x4 kept(f32x4 z, int dtype) {
-    if (dtype == DETBOX_F16) {
+__device__ inline f32x4 kept(f32x4 z, bool half) {
+    if (half) {
 #pragma unroll
-        for (int j = 0; j < 4; ++j) z[j] = z[j] > 0.f && z[j] < 0x1p-24f ? 0x1p-24f : z[j];
+        for (int j = 0; j < 4; ++j) z[j] = z[j] > 0.f ? fmaxf(z[j], 0x1p-24f) : z[j];
     }
     return z;
 }
@@ -152,7 +152,7 @@ __device__ inline void finish4(const Epilogue &ep, int64_t row, int64_t res_row,
     if (left <= 0) return;
     if (ep.unscale) z *= *ep.unscale;
     if (ep.bias) z += load4(ep.bias, ep.bias_dtype, n, left);
-    if (ep.pre) store4(ep.pre, ep.pre_dtype, row + n, left, kept(z, ep.pre_dtype));
+    if (ep.pre) store4(ep.pre, ep.pre_dtype, row + n, left, kept(z, ep.pre_dtype == DETBOX_F16));
     if (ep.act != DETBOX_ACTIVATION_NONE) z = act4(z, ep.act);
     if (ep.residual) z += load4(ep.residual, ep.out_dtype, res_row + n, left);
     store4(ep.out, ep.out_dtype, row + n, left, z);
@@ -491,7 +491,7 @@ __global__ __launch_bounds__((BM / WM) * (BN / WN) * 64) void gemm_kernel(GemmAr
                 }
                 if constexpr (UNSCALE) z *= unscale;
                 z += bias;
-                if (g.ep.pre) store4(g.ep.pre, g.ep.pre_dtype, at, left, kept(z, g.ep.pre_dtype));
+                if (g.ep.pre) store4(g.ep.pre, g.ep.pre_dtype, at, left, kept(z, std::is_same_v<T, _Float16>));
                 if (g.ep.act != DETBOX_ACTIVATION_NONE) z = act4(z, g.ep.act);
                 if (g.ep.residual)
                     z += left == 4 ? widen4(raw[u], g.ep.out_dtype)
