@@ -156,8 +156,6 @@ void refuse_tangents(const char *name, std::initializer_list<const MaybeTensor *
         }
 }
 
-Tensor value(const MaybeTensor &t) { return t.has_value() ? *t : Tensor(); }
-
 // ---- layer_norm ----------------------------------------------------------------------------------------------------------
 
 struct NormResult { Tensor y, m, weight, stats; };

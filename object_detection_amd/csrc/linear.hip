@@ -7,9 +7,10 @@
 // which the products take out again: a mean over many rows has gradients below fp16's smallest step, a scaled loss some beyond
 // its largest value.
 //
-// Bounds: a long contraction is bound by the matrix instructions (8192^3 bf16 1.25-1.31 PFLOP/s in all three products), a short
-// one by memory (RetinaNet's class logits, 480348 x 256 bf16 by 81, fp32 out: 88-97 us = 4.1-4.6 TB/s), few rows by the read of the
-// weight (4 x 4096 by 4096: 9 us = 3.7 TB/s).
+// Bounds: a long contraction is bound by the matrix instructions (8192^3 bf16, 20 training steps in a row:
+// 1.15-1.19 PFLOP/s on average in all three products, 1.24-1.28 at best), a short
+// one by memory (RetinaNet's class logits, 480348 x 256 bf16 by 81, fp32 out: 97 us = 4.2 TB/s), few rows by the read of the
+// weight and its latency (4 x 4096 by 4096: 9.8 us = 3.4 TB/s).
 //
 // One tile kernel serves all three products.  Each operand lies in memory either along the contraction (x, W forward) or
 // across it (W in grad_x; dz and x in grad_W); both come into LDS as they lie, 16 bytes at a time, and only the read of a
@@ -318,8 +319,8 @@ __device__ inline void job_of(int wg, int tiles_m, int tiles_n, int splits, int 
 // The products of one step, from the buffer `cur` (A's rows first), while the next step comes into `nxt`.  The two pointers
 // are restrict: without it the compiler takes every LDS read for one that may want what is still on its way and waits for
 // the whole transfer first.  Reads and matrix instructions are interleaved by hand, the second half's reads under the first
-// half's products.  8192^3 bf16 forward: 997 us with staging through registers, 944 with the compiler's order, 860 so =
-// 1.28 PFLOP/s (grad_x 1.30, grad_W 1.31).
+// half's products.  8192^3 bf16 forward, short runs: 997 us with staging through registers, 944 with the compiler's order, 860 so;
+// over 20 training steps in a row 927-937 on average.
 template <typename T, bool AX, bool BX, int BM, int BN, int FM, int FN>
 __device__ __forceinline__ void multiply_step(const char *__restrict__ cur, int wm, int wn, f32x4 (&acc)[FM][FN]) {
 #pragma unroll
@@ -646,7 +647,7 @@ __global__ __launch_bounds__(256) void linear_slope_kernel(const void *g, int gd
 
 // At most 16 MT rows of x (serving): the weight is all there is to read, and it goes straight into registers, once.  A workgroup
 // owns 16 columns; its eight waves take the contraction's packs in turn and add their sums in LDS in order.  No second launch.
-// 4 x 4096 by 4096 bf16: 11.1 us as tiles in pieces and their join, 9.2 us = 3.7 TB/s so.
+// 4 x 4096 by 4096 bf16: 11.1 us as tiles in pieces and their join, 9.2-9.8 us = 3.4-3.6 TB/s so.
 constexpr int64_t FEW_ROWS = 64;
 constexpr int FEW_BLOCK = 512, FEW_WAVES = FEW_BLOCK / 64;
 
@@ -715,7 +716,8 @@ __global__ __launch_bounds__(FEW_BLOCK) void gemm_few_kernel(const Operand<T> a,
 bool act_ok(int act) { return act >= DETBOX_ACTIVATION_NONE && act <= DETBOX_ACTIVATION_SIGMOID; }
 
 // How a product is cut.  Tiles of 256 x 256 (eight waves of 128 x 64, one workgroup per CU) where they alone fill the chip and
-// have steps enough to hide their start and end; tiles of 128 rows (eight waves, two or three workgroups per CU) otherwise,
+// have steps enough to hide their start and end; tiles of 128 rows (eight waves; two workgroups per CU at widths of 128 and 96,
+// three at 64, by their LDS) otherwise,
 // as wide as the columns ask for, with the contraction in pieces where there are fewer than two tiles per CU.  Measured (bf16
 // unless it says fp32, us, large / small): 8192^3 860 / 1043, 4096^3 115 / 132, 8192 x 1024 by 8192 149 / 153, 8192 x 512 by
 // 8192 103 / 95, 65536 x 256 by 256 24 / 21, 2048^3 (64 large tiles) 59 / 31.  Width (128 / as wide as needed): 480348 x 64 by
@@ -877,6 +879,7 @@ extern "C" int detbox_linear_forward(int dtype, int activation, const void *x, i
 
 extern "C" size_t detbox_linear_backward_workspace_bytes(int dtype, int activation, int grad_dtype, int64_t M, int64_t N, int64_t K) {
     if (!dtype_ok(dtype) || M < 0 || N < 1 || K < 1) return 0;
+    // dz has its place in every case: whether g can be used as it lies depends on its address and stride too
     (void)activation; (void)grad_dtype;
     const int64_t vec = 16 / (int64_t)dtype_size(dtype), ldz = (N + vec - 1) / vec * vec;
     size_t b = align_up((size_t)slices_of(M, N).count * (size_t)N * sizeof(float), 256);

@@ -8,7 +8,8 @@
 // Every logit is read once in each direction.  Rows of up to 2048 logits live in the registers of 4, 16 or 64 lanes; longer
 // rows are streamed with a running maximum and sums that are rescaled when the maximum grows, by one workgroup per row or,
 // when there are few rows, by several whose partial results a second launch joins.  HBM bound: 4096 rows of 131071 bf16 logits
-// 161-188 us forward = 5.7-6.7 TB/s, 350 us backward = 6.1 TB/s; 480348 rows of 81 fp32 logits 41 + 67 us.
+// 188 us forward = 5.7 TB/s, 358 us backward = 6.0 TB/s; 480348 rows of 81 fp32 logits 41 + 67 us.  With alternatives the 16-bit
+// form of long rows takes 116-118 registers and 48 bytes of scratch per lane: four waves per SIMD, eight without.
 #include "dtype.h"
 
 using namespace detbox;

@@ -56,9 +56,10 @@ class _BoxOps:
 
     def head_logits(self, features: torch.Tensor, embeddings: torch.Tensor, bias: Optional[torch.Tensor] = None,
                     tower: Sequence[tuple] = (), activation: str = 'relu') -> torch.Tensor:
-        """Class logits [B,P,C] in fp32 from one feature vector per anchor or point: the `out_confs` that loss, pre_predict
-        and detect take, for heads that score classes by embeddings (the reference's heads end in a convolution instead,
-        src/models/retinanet.py:100-106).  features [B,P,D], embeddings [C,D] with C = self.nc, bias [C];
+        """Class logits [B,P,C] in fp32 from one feature vector per anchor or point, for heads that score classes by embeddings
+        (the reference's heads end in a convolution instead, src/models/retinanet.py:100-106).  They are the `out_confs` that loss,
+        pre_predict and detect take, whose own limits stay: at most 128 selected classes there, 256 in the focal loss.  Beyond those,
+        ops.label_log_probs takes the logits (training loss, confidence, alternatives), at any number of classes.  features [B,P,D], embeddings [C,D] with C = self.nc, bias [C];
         tower: layers (norm_weight, norm_bias, weight, bias) with weight [D,D], each
             features = activation(layer_norm(features) weight^T + bias) + features
         Differentiable in everything but the choice of activation."""
