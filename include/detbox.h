@@ -167,7 +167,7 @@ int detbox_smooth_l1_masked_backward(const float *input, const float *target, co
 
 #define DETBOX_ACTIVATION_NONE 0
 #define DETBOX_ACTIVATION_RELU 1
-#define DETBOX_ACTIVATION_GELU 2    /* z * Phi(z), Phi the normal distribution function to 7.5e-8 */
+#define DETBOX_ACTIVATION_GELU 2    /* z * Phi(z), Phi the normal distribution function, within 3e-7 */
 #define DETBOX_ACTIVATION_SILU 3    /* z * sigmoid(z) */
 #define DETBOX_ACTIVATION_SIGMOID 4
 

@@ -7,10 +7,9 @@
 // which the products take out again: a mean over many rows has gradients below fp16's smallest step, a scaled loss some beyond
 // its largest value.
 //
-// Bounds: a long contraction is bound by the matrix instructions (8192^3 bf16, 20 training steps in a row:
-// 1.15-1.19 PFLOP/s on average in all three products, 1.24-1.28 at best), a short
-// one by memory (RetinaNet's class logits, 480348 x 256 bf16 by 81, fp32 out: 97 us = 4.2 TB/s), few rows by the read of the
-// weight and its latency (4 x 4096 by 4096: 9.8 us = 3.4 TB/s).
+// Bounds: a long contraction is bound by the matrix instructions (8192^3 bf16, 20 training steps in a row: 1.15-1.19
+// PFLOP/s on average in all three products, 1.24-1.28 at best), a short one by memory (RetinaNet's class logits, 480348 x 256
+// bf16 by 81, fp32 out: 97 us = 4.2 TB/s), few rows by the read of the weight and its latency (4 x 4096 by 4096: 9.8 us = 3.4 TB/s).
 //
 // One tile kernel serves all three products.  Each operand lies in memory either along the contraction (x, W forward) or
 // across it (W in grad_x; dz and x in grad_W); both come into LDS as they lie, 16 bytes at a time, and only the read of a
@@ -29,7 +28,8 @@ typedef void __attribute__((address_space(3))) *lptr_t;
 
 __device__ inline float sigmoid_f(float z) { return __builtin_amdgcn_rcpf(1.0f + fast_exp(-z)); }
 
-// Normal distribution function by Abramowitz and Stegun, Handbook of Mathematical Functions, 7.1.26 (error below 1.5e-7 / 2);
+// Normal distribution function by Abramowitz and Stegun, Handbook of Mathematical Functions, 7.1.26 (error below 1.5e-7 / 2, 2.8e-7
+// at most as measured in fp32 arithmetic, on [-8, 8]);
 // e is exp(-z^2 / 2), which the slope needs as well.
 __device__ inline float normal_cdf(float z, float e) {
     const float u = fabsf(z) * 0.70710678118654752f;
@@ -600,7 +600,8 @@ __device__ inline int scale_exponent(const float *peaks, int count) {
 }
 
 // dz = g * act'(pre) in the type of x with rows of ldz elements (zeros behind N), and partial column sums of the unrounded dz
-// per row slice.  With peaks, dz is stored times their power of two, the inverse of which goes to *unscale.  LANES lanes share a row, four columns each; HBM bound (16384 x 4096 bf16 with gelu: 96 us = 4.2 TB/s).
+// per row slice.  With peaks, dz is stored times their power of two, the inverse of which goes to *unscale.
+// LANES lanes share a row, four columns each; HBM bound (16384 x 4096 bf16 with gelu: 96 us = 4.2 TB/s).
 template <typename T, int LANES>
 __global__ __launch_bounds__(256) void linear_slope_kernel(const void *g, int gdt, int64_t ldg, const T *__restrict__ pre, int act,
                                                            int64_t M, int64_t N, int64_t ldz, int64_t rows_per_slice,

@@ -5,9 +5,9 @@
 //
 // HBM bound (240174 x 1024 bf16: forward 225 us = 4.4 TB/s, backward 271 us = 5.4 TB/s); a single row is bound by latency, its
 // parameters and its elements one after the other (1 x 1024: 6 us).  A row lives in the registers of a group of 4, 16, 64, 256, 512
-// or 1024 lanes, 8 or 16 elements each, so that it is read once and the deviations are squared about the mean itself.  A lane keeps the parameters of its columns, and in the
-// backward pass their gradients, in registers over all the rows its group takes; the groups' sums meet in LDS, the
-// workgroups' in the workspace.  Rows of more than 16384 elements are walked three times.
+// or 1024 lanes, 8 or 16 elements each, so that it is read once and the deviations are squared about the mean itself.
+// A lane keeps the parameters of its columns, and in the backward pass their gradients, in registers over all the rows its group
+// takes; the groups' sums meet in LDS, the workgroups' in the workspace.  Rows of more than 16384 elements are walked three times.
 #include "columns.h"
 
 using namespace detbox;

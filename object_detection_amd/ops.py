@@ -559,7 +559,7 @@ def linear(x: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Tensor] =
     out_dtype=torch.float32, the fp32 sum itself (the logits select_decode and focal_loss_sum take).  Differentiable in x,
     weight, bias and residual; products are summed in fp32, the gradient at the activation's input is rounded to the type
     of x before it is multiplied (float16: scaled into range by a power of two first, so that gradients far below or above
-    that type's range count too).  The normal distribution function of gelu is off by at most 7.5e-8, in float32 too."""
+    that type's range count too).  gelu takes the normal distribution function within 3e-7, in float32 too."""
     act = ACTIVATIONS.get(activation)
     if act is None:
         raise ValueError(f'linear: unknown activation {activation!r}')
